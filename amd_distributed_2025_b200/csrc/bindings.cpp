@@ -17,6 +17,8 @@
 #include <string>
 #include <vector>
 
+#include "bindings_common.h"
+#include "bindings_experts.h"
 #include "fp8_gemm.h"
 #include "gemm_rs.h"
 #include "host_ops.h"
@@ -28,41 +30,12 @@
 
 namespace py = pybind11;
 using b200::SymmHeap;
+using namespace b200::bind;
 
 namespace {
 
-void cuda_check(cudaError_t e, const char* what) {
-  TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
-}
-
-// A kernel can read device memory and pinned host memory; an ordinary host tensor would fault the GPU.
-void check_reachable(const at::Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda() || t.is_pinned(), what, " must be a CUDA tensor");
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kHalf: return 0;
-    case at::kBFloat16: return 1;
-    case at::kFloat: return 2;
-    default: TORCH_CHECK(false, "unsupported dtype ", t, " (expected float16, bfloat16 or float32)");
-  }
-  return -1;
-}
-
 void fill_peer_bases(const SymmHeap& heap, uint64_t* out) {
   for (int r = 0; r < b200::kMaxWorldSize; ++r) out[r] = r < heap.world_size() ? heap.peer_base(r) : 0;
-}
-
-py::dict status_to_dict(const b200::StatusWord& w) {
-  py::dict d;
-  d["code"] = w.code;
-  d["phase"] = w.phase;
-  d["peer"] = w.peer;
-  d["detail"] = w.detail;
-  d["epoch"] = w.epoch;
-  d["seen"] = w.seen;
-  return d;
 }
 
 at::Tensor heap_view(SymmHeap& heap, int64_t offset, std::vector<int64_t> shape, at::ScalarType dtype) {
@@ -874,48 +847,6 @@ class GemmRsEngine {
 
 // ------------------------------------------------------------------------ fp8 GEMM ----
 
-int device_sms(int device) {
-  static const std::vector<int> sms = [] {
-    std::vector<int> v;
-    for (int d = 0; d < (int)at::cuda::device_count(); ++d)
-      v.push_back(at::cuda::getDeviceProperties(d)->multiProcessorCount);
-    return v;
-  }();
-  return sms.at((size_t)device);
-}
-
-// Where fp8_gemm leaves the record of an expired wait: one word per device, in mapped host memory, for the life of the
-// process (the operation has no object of its own to hold it).
-b200::StatusWord* fp8_status(int device) {
-  constexpr int kDevices = 64;
-  static b200::StatusWord* const words = [] {
-    // (the first call may come while a stream is being captured, which an allocation would break off in any other mode)
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "fp8_gemm status");
-    void* w = nullptr;
-    const cudaError_t e = cudaHostAlloc(&w, kDevices * sizeof(b200::StatusWord), cudaHostAllocMapped | cudaHostAllocPortable);
-    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "fp8_gemm status");
-    cuda_check(e, "fp8_gemm status");
-    std::memset(w, 0, kDevices * sizeof(b200::StatusWord));
-    return static_cast<b200::StatusWord*>(w);
-  }();
-  TORCH_CHECK(device >= 0 && device < kDevices, "device index out of range");
-  return words + device;
-}
-
-uint32_t fp8_status_code(int device) { return reinterpret_cast<const volatile b200::StatusWord*>(fp8_status(device))->code; }
-
-// The record of a device, which is cleared: an expired wait leaves nothing behind that a later call could trip over.
-py::dict fp8_gemm_take_status(int device) {
-  b200::StatusWord* w = fp8_status(device);
-  const uint32_t code = fp8_status_code(device);
-  std::atomic_thread_fence(std::memory_order_acquire);
-  b200::StatusWord copy = *w;
-  copy.code = code;
-  if (code != 0) std::memset(w, 0, sizeof(*w));
-  return status_to_dict(copy);
-}
-
 void run_fp8_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_scale, const at::Tensor& b_scale,
                   const at::Tensor& c, int64_t timeout_ns) {
   b200::Fp8GemmArgs g;
@@ -991,37 +922,6 @@ c10::optional<at::Tensor> fp8_gemm_try(const at::Tensor& a, const at::Tensor& b,
 // and what Python does around the call of a layer 0.7 us, beside 1.9 us for the launch.  (Host time a call, us: forward
 // 4.8, now 4.1; dispatch + combine 6.6, now 5.7; gemm_rs 4.8, now 4.4; fp8_gemm 5.3, now 4.2.)
 
-const at::Tensor& tensor_arg(PyObject* o) {
-  if (!THPVariable_Check(o)) throw py::type_error(std::string("expected a torch.Tensor, got ") + Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
-}
-void count_args(Py_ssize_t got, Py_ssize_t want) {
-  if (got != want) throw py::type_error("expected " + std::to_string(want) + " arguments, got " + std::to_string(got));
-}
-double double_arg(PyObject* o) {
-  const double v = PyFloat_AsDouble(o);
-  if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
-  return v;
-}
-PyObject* wrap(const c10::optional<at::Tensor>& t) {
-  if (!t.has_value()) Py_RETURN_NONE;
-  return THPVariable_Wrap(*t);
-}
-// Runs a call; a C++ exception becomes a Python one.
-template <typename F>
-PyObject* guarded(F&& call) {
-  HANDLE_TH_ERRORS
-  try {
-    return call();
-  } catch (py::error_already_set& e) {
-    e.restore();
-    return nullptr;
-  } catch (py::builtin_exception& e) {
-    e.set_error();
-    return nullptr;
-  }
-  END_HANDLE_TH_ERRORS
-}
 template <typename T>
 T& native(PyObject* o) {
   return *py::handle(o).cast<T*>();
@@ -1698,6 +1598,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_rs", &gemm_rs);
   m.def("fp8_gemm", &fp8_gemm);
   if (PyModule_AddFunctions(m.ptr(), kModuleCalls) != 0) throw py::error_already_set();
+  b200::bind_experts(m);
   m.def("fp8_gemm_take_status", &fp8_gemm_take_status);
   m.def("fp8_wait_selftest", [](int device, int64_t timeout_ns) {
     c10::cuda::CUDAGuard guard(device);

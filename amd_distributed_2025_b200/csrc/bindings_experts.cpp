@@ -1,0 +1,376 @@
+// Python calls of the operators around a GPU's experts: rows with block scales (fp8_rows.h), tokens sorted by expert
+// (moe_sort.h).  Shapes and types are looked at before devices, so that a wrong call is refused without a GPU too.
+#include "bindings_experts.h"
+
+#include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
+
+#include <unordered_set>
+
+#include "bindings_common.h"
+#include "fp8_rows.h"
+#include "moe_sort.h"
+
+namespace {
+
+using namespace b200::bind;
+using c10::optional;
+
+optional<at::Tensor> optional_arg(PyObject* o) {
+  if (o == Py_None) return c10::nullopt;
+  return tensor_arg(o);
+}
+int64_t int_arg(PyObject* o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw py::error_already_set();
+  return v;
+}
+bool bool_arg(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw py::error_already_set();
+  return v != 0;
+}
+PyObject* tuple_of(std::initializer_list<optional<at::Tensor>> items) {
+  PyObject* t = PyTuple_New((Py_ssize_t)items.size());
+  if (t == nullptr) throw py::error_already_set();
+  Py_ssize_t i = 0;
+  for (const auto& item : items) PyTuple_SET_ITEM(t, i++, wrap(item));
+  return t;
+}
+
+void check_device(const at::Tensor& t, const at::Tensor& first, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor");
+  TORCH_CHECK(t.get_device() == first.get_device(), what, " must be on the device of the other tensors (", first.device().str(),
+              "), not on ", t.device().str());
+}
+
+// A matrix whose rows are contiguous; the distance between them is free (0: the same row again).
+at::Tensor with_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+int64_t row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
+}
+
+// ------------------------------------------------------------- rows with block scales ----
+
+void check_no_gradient(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), what,
+              " requires a gradient, and this operator has none: call it under torch.no_grad()");
+}
+
+// (x, weight, eps, residual or None, total_out or None, normed) -> (q, scale, total or None, normed or None)
+PyObject* rms_norm_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count_args(n, 6);
+    const at::Tensor& x_in = tensor_arg(v[0]);
+    const at::Tensor& weight_in = tensor_arg(v[1]);
+    const double eps = double_arg(v[2]);
+    const optional<at::Tensor> residual_in = optional_arg(v[3]);
+    optional<at::Tensor> total = optional_arg(v[4]);
+    const bool want_normed = bool_arg(v[5]);
+    TORCH_CHECK(x_in.dim() == 2, "x must be a matrix [rows, columns]");
+    const int64_t rows = x_in.size(0), cols = x_in.size(1);
+    const auto type = x_in.scalar_type();
+    const int code = dtype_code(type);
+    TORCH_CHECK(cols >= 1 && cols <= b200::kMaxNormCols, "x must have 1 to ", num(b200::kMaxNormCols), " columns, not ", num(cols));
+    TORCH_CHECK(weight_in.dim() == 1 && weight_in.size(0) == cols, "weight must be a vector of ", num(cols), " values");
+    TORCH_CHECK(weight_in.scalar_type() == type || weight_in.scalar_type() == at::kFloat, "weight must have x's type or be float32");
+    TORCH_CHECK(std::isfinite(eps) && eps >= 0, "eps must not be negative");
+    check_no_gradient(x_in, "x");
+    check_no_gradient(weight_in, "weight");
+    if (residual_in) {
+      TORCH_CHECK(residual_in->sizes() == x_in.sizes() && residual_in->scalar_type() == type, "residual must have x's shape and type");
+      check_no_gradient(*residual_in, "residual");
+    }
+    TORCH_CHECK(!total || residual_in, "total_out is the sum of x and residual: there is no residual");
+    if (total) {
+      TORCH_CHECK(total->sizes() == x_in.sizes() && total->scalar_type() == type, "total_out must have x's shape and type");
+      TORCH_CHECK((cols == 1 || total->stride(1) == 1) && (rows <= 1 || total->stride(0) >= cols),
+                  "total_out must have contiguous rows that do not overlap");
+      check_no_gradient(*total, "total_out");
+    }
+    TORCH_CHECK(x_in.is_cuda(), "x must be a CUDA tensor");
+    check_device(weight_in, x_in, "weight");
+    if (residual_in) check_device(*residual_in, x_in, "residual");
+    if (total) {
+      check_device(*total, x_in, "total_out");
+      // (the very same rows are fine: a lane reads its columns before it writes them)
+      at::assert_no_partial_overlap(*total, x_in);
+      at::assert_no_partial_overlap(*total, *residual_in);
+      at::assert_no_overlap(*total, weight_in);
+    }
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = with_rows(x_in), weight = weight_in.contiguous();
+    at::Tensor residual;
+    if (residual_in) {
+      residual = with_rows(*residual_in);
+      if (!total) total = new_cuda({rows, cols}, type, x);
+    }
+    const at::Tensor q = new_cuda({rows, cols}, at::kFloat8_e4m3fn, x);
+    const at::Tensor scale = new_cuda({rows, (cols + 127) / 128}, at::kFloat, x);
+    optional<at::Tensor> normed;
+    if (want_normed) normed = new_cuda({rows, cols}, type, x);
+    b200::RmsNormFp8Args a = {};
+    a.x = x.const_data_ptr();
+    a.residual = residual_in ? residual.const_data_ptr() : nullptr;
+    a.weight = weight.const_data_ptr();
+    a.total = total ? total->mutable_data_ptr() : nullptr;
+    a.normed = normed ? normed->mutable_data_ptr() : nullptr;
+    a.q = q.mutable_data_ptr();
+    a.scale = scale.mutable_data_ptr<float>();
+    a.rows = rows;
+    a.cols = (int32_t)cols;
+    a.x_stride = row_stride(x);
+    a.residual_stride = residual_in ? row_stride(residual) : 0;
+    a.total_stride = total ? row_stride(*total) : 0;
+    a.eps = (float)eps;
+    a.dtype = code;
+    a.weight_dtype = dtype_code(weight.scalar_type());
+    cuda_check(b200::launch_rms_norm_fp8(a, device_sms(x.get_device()), at::cuda::getCurrentCUDAStream()), "rms_norm_fp8 launch");
+    return tuple_of({q, scale, total, normed});
+  });
+}
+
+PyObject* silu_mul_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {  // (x) -> (q, scale)
+  return guarded([&] {
+    count_args(n, 1);
+    const at::Tensor& x_in = tensor_arg(v[0]);
+    TORCH_CHECK(x_in.dim() == 2, "x must be a matrix [rows, 2 columns]");
+    TORCH_CHECK(x_in.size(1) >= 2 && x_in.size(1) % 2 == 0 && x_in.size(1) / 2 <= INT32_MAX - 256,
+                "x must have an even number of columns: gates, then the values that they multiply");
+    const int64_t rows = x_in.size(0), cols = x_in.size(1) / 2;
+    const int code = dtype_code(x_in.scalar_type());
+    check_no_gradient(x_in, "x");
+    TORCH_CHECK(x_in.is_cuda(), "x must be a CUDA tensor");
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = with_rows(x_in);
+    const at::Tensor q = new_cuda({rows, cols}, at::kFloat8_e4m3fn, x);
+    const at::Tensor scale = new_cuda({rows, (cols + 127) / 128}, at::kFloat, x);
+    b200::SiluMulFp8Args a = {};
+    a.x = x.const_data_ptr();
+    a.q = q.mutable_data_ptr();
+    a.scale = scale.mutable_data_ptr<float>();
+    a.rows = rows;
+    a.cols = (int32_t)cols;
+    a.x_stride = row_stride(x);
+    a.dtype = code;
+    cuda_check(b200::launch_silu_mul_fp8(a, device_sms(x.get_device()), at::cuda::getCurrentCUDAStream()), "silu_mul_fp8 launch");
+    return tuple_of({q, scale});
+  });
+}
+
+// -------------------------------------------------------------- tokens sorted by expert ----
+
+constexpr int64_t kMaxEntries = int64_t(1) << 30;
+
+int64_t check_entries(int64_t tokens, int64_t k) {
+  TORCH_CHECK(k >= 1 && k <= b200::kSortMaxTopk, "a token must have 1 to ", num(b200::kSortMaxTopk), " experts, not ", num(k));
+  TORCH_CHECK(tokens <= kMaxEntries / k, "more than 2^30 (token, expert) entries");
+  return tokens * k;
+}
+
+// (x, indices, num_experts, scale or None) -> (rows, rows_scale or None, offsets, row_of)
+PyObject* sort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count_args(n, 4);
+    const at::Tensor& x_in = tensor_arg(v[0]);
+    const at::Tensor& indices_in = tensor_arg(v[1]);
+    const int64_t experts = int_arg(v[2]);
+    const optional<at::Tensor> scale_in = optional_arg(v[3]);
+    TORCH_CHECK(x_in.dim() == 2 && x_in.size(1) >= 1, "x must be a matrix [tokens, hidden]");
+    const auto type = x_in.scalar_type();
+    if (type != at::kFloat8_e4m3fn) dtype_code(type);
+    const int64_t tokens = x_in.size(0), hidden = x_in.size(1);
+    TORCH_CHECK(hidden <= INT32_MAX / 8, "hidden is too large");
+    TORCH_CHECK(indices_in.dim() == 2 && indices_in.size(0) == tokens, "indices must be [tokens, experts per token]");
+    TORCH_CHECK(indices_in.scalar_type() == at::kInt || indices_in.scalar_type() == at::kLong, "indices must be int32 or int64");
+    const int64_t k = indices_in.size(1);
+    const int64_t entries = check_entries(tokens, k);
+    TORCH_CHECK(experts >= 1 && experts <= b200::kSortMaxExperts, "num_experts must be 1 to ", num(b200::kSortMaxExperts), ", not ", num(experts));
+    if (scale_in) {
+      TORCH_CHECK(scale_in->dim() == 2 && scale_in->size(0) == tokens && scale_in->size(1) >= 1 &&
+                      scale_in->size(1) <= INT32_MAX / 8 && scale_in->scalar_type() == at::kFloat,
+                  "scale must be float32 [tokens, scales of a row]");
+    }
+    TORCH_CHECK(x_in.is_cuda(), "x must be a CUDA tensor");
+    check_device(indices_in, x_in, "indices");
+    if (scale_in) check_device(*scale_in, x_in, "scale");
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = with_rows(x_in), indices = indices_in.contiguous();
+    const at::Tensor rows = new_cuda({entries, hidden}, type, x);
+    const at::Tensor offsets = new_cuda({experts + 1}, at::kInt, x), row_of = new_cuda({tokens, k}, at::kInt, x);
+    at::Tensor scale, work;
+    optional<at::Tensor> rows_scale;
+    b200::SortTokensArgs a = {};
+    if (scale_in) {
+      scale = with_rows(*scale_in);
+      rows_scale = new_cuda({entries, scale.size(1)}, at::kFloat, x);
+      a.scale = scale.const_data_ptr<float>();
+      a.rows_scale = rows_scale->mutable_data_ptr<float>();
+      a.scale_stride = row_stride(scale);
+      a.scale_cols = (int32_t)scale.size(1);
+    }
+    if (const int64_t words = b200::sort_tokens_work(tokens, (int)k, (int)experts)) {
+      work = new_cuda({words}, at::kInt, x);
+      a.work = work.mutable_data_ptr<int32_t>();
+    }
+    a.x = x.const_data_ptr();
+    a.indices = indices.const_data_ptr();
+    a.rows = rows.mutable_data_ptr();
+    a.offsets = offsets.mutable_data_ptr<int32_t>();
+    a.row_of = row_of.mutable_data_ptr<int32_t>();
+    a.elem_bytes = (int32_t)x.element_size();
+    a.x_stride = row_stride(x) * a.elem_bytes;
+    a.row_bytes = hidden * a.elem_bytes;
+    a.tokens = (int32_t)tokens;
+    a.k = (int32_t)k;
+    a.experts = (int32_t)experts;
+    a.wide_ids = indices.scalar_type() == at::kLong;
+    cuda_check(b200::launch_sort_tokens(a, device_sms(x.get_device()), at::cuda::getCurrentCUDAStream()), "sort_tokens launch");
+    return tuple_of({rows, rows_scale, offsets, row_of});
+  });
+}
+
+void check_order(const at::Tensor& row_of, const char* what) {
+  TORCH_CHECK(row_of.dim() == 2 && row_of.scalar_type() == at::kInt, what, " must be int32 [tokens, experts per token]");
+}
+
+at::Tensor weights_of(const at::Tensor& w, const at::Tensor& row_of) {
+  TORCH_CHECK(w.sizes() == row_of.sizes() && w.scalar_type() == at::kFloat, "weights must be float32 [tokens, experts per token]");
+  return w;
+}
+
+// (rows, row_of, weights or None) -> out
+PyObject* unsort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count_args(n, 3);
+    const at::Tensor& rows_in = tensor_arg(v[0]);
+    const at::Tensor& row_of_in = tensor_arg(v[1]);
+    const optional<at::Tensor> weights_in = optional_arg(v[2]);
+    TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(1) >= 1 && rows_in.size(1) <= INT32_MAX / 8, "rows must be a matrix [rows, hidden]");
+    const int code = dtype_code(rows_in.scalar_type());
+    check_order(row_of_in, "row_of");
+    const int64_t tokens = row_of_in.size(0), k = row_of_in.size(1), hidden = rows_in.size(1);
+    TORCH_CHECK(rows_in.size(0) == check_entries(tokens, k), "rows must have a row for each of the ", num(tokens * k), " entries, not ",
+                num(rows_in.size(0)));
+    if (weights_in) weights_of(*weights_in, row_of_in);
+    TORCH_CHECK(rows_in.is_cuda(), "rows must be a CUDA tensor");
+    check_device(row_of_in, rows_in, "row_of");
+    if (weights_in) check_device(*weights_in, rows_in, "weights");
+    c10::cuda::CUDAGuard guard(rows_in.device());
+    const at::Tensor rows = with_rows(rows_in), row_of = row_of_in.contiguous();
+    at::Tensor weights;
+    if (weights_in) weights = weights_in->contiguous();
+    at::Tensor out = new_cuda({tokens, hidden}, rows.scalar_type(), rows);
+    b200::UnsortTokensArgs a = {};
+    a.rows = rows.const_data_ptr();
+    a.weights = weights_in ? weights.const_data_ptr<float>() : nullptr;
+    a.row_of = row_of.const_data_ptr<int32_t>();
+    a.out = out.mutable_data_ptr();
+    a.rows_stride = row_stride(rows) * (int64_t)rows.element_size();
+    a.num_rows = rows.size(0);
+    a.tokens = (int32_t)tokens;
+    a.k = (int32_t)k;
+    a.hidden = (int32_t)hidden;
+    a.dtype = code;
+    cuda_check(b200::launch_unsort_tokens(a, device_sms(rows.get_device()), at::cuda::getCurrentCUDAStream()), "unsort_tokens launch");
+    return wrap(out);
+  });
+}
+
+// (grad, rows, offsets, row_of, weights or None, want_rows, want_weights) -> (grad_rows or None, grad_weights or None)
+PyObject* unsort_tokens_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count_args(n, 7);
+    const at::Tensor& grad_in = tensor_arg(v[0]);
+    const at::Tensor& rows_in = tensor_arg(v[1]);
+    const at::Tensor& offsets_in = tensor_arg(v[2]);
+    const at::Tensor& row_of_in = tensor_arg(v[3]);
+    const optional<at::Tensor> weights_in = optional_arg(v[4]);
+    const bool want_rows = bool_arg(v[5]), want_weights = bool_arg(v[6]) && weights_in;
+    const auto type = rows_in.scalar_type();
+    const int code = dtype_code(type);
+    check_order(row_of_in, "row_of");
+    TORCH_CHECK(offsets_in.dim() == 1 && offsets_in.size(0) >= 2 && offsets_in.scalar_type() == at::kInt, "offsets must be int32 [num_experts + 1]");
+    const int64_t tokens = row_of_in.size(0), k = row_of_in.size(1);
+    TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(1) >= 1 && rows_in.size(1) <= INT32_MAX / 8 &&
+                    rows_in.size(0) == check_entries(tokens, k),
+                "rows must have a row for each of the ", num(tokens * k), " entries");
+    const int64_t hidden = rows_in.size(1), entries = tokens * k;
+    TORCH_CHECK(grad_in.dim() == 2 && grad_in.size(0) == tokens && grad_in.size(1) == hidden && grad_in.scalar_type() == type,
+                "the gradient must be [tokens, hidden] of the rows' type");
+    if (weights_in) weights_of(*weights_in, row_of_in);
+    TORCH_CHECK(rows_in.is_cuda(), "rows must be a CUDA tensor");
+    check_device(grad_in, rows_in, "the gradient");
+    check_device(offsets_in, rows_in, "offsets");
+    check_device(row_of_in, rows_in, "row_of");
+    if (weights_in) check_device(*weights_in, rows_in, "weights");
+    c10::cuda::CUDAGuard guard(rows_in.device());
+    optional<at::Tensor> grad_rows, grad_weights;
+    if (want_rows) grad_rows = new_cuda({entries, hidden}, type, rows_in);
+    if (want_weights) grad_weights = new_cuda({tokens, k}, at::kFloat, rows_in);
+    if (!want_rows && !want_weights) return tuple_of({grad_rows, grad_weights});
+    const at::Tensor grad = with_rows(grad_in), offsets = offsets_in.contiguous(), row_of = row_of_in.contiguous();
+    at::Tensor rows, weights;
+    if (want_weights) rows = with_rows(rows_in);
+    if (weights_in) weights = weights_in->contiguous();
+    b200::UnsortBackwardArgs a = {};
+    a.grad = grad.const_data_ptr();
+    a.rows = want_weights ? rows.const_data_ptr() : nullptr;
+    a.weights = weights_in ? weights.const_data_ptr<float>() : nullptr;
+    a.row_of = row_of.const_data_ptr<int32_t>();
+    a.end = offsets.const_data_ptr<int32_t>() + offsets.size(0) - 1;
+    a.grad_rows = want_rows ? grad_rows->mutable_data_ptr() : nullptr;
+    a.grad_weights = want_weights ? grad_weights->mutable_data_ptr<float>() : nullptr;
+    a.grad_stride = row_stride(grad) * (int64_t)grad.element_size();
+    a.rows_stride = want_weights ? row_stride(rows) * (int64_t)rows.element_size() : 0;
+    a.num_rows = entries;
+    a.tokens = (int32_t)tokens;
+    a.k = (int32_t)k;
+    a.hidden = (int32_t)hidden;
+    a.dtype = code;
+    cuda_check(b200::launch_unsort_tokens_backward(a, device_sms(rows_in.get_device()), at::cuda::getCurrentCUDAStream()),
+               "unsort_tokens_backward launch");
+    return tuple_of({grad_rows, grad_weights});
+  });
+}
+
+// While the current stream is being captured: whether a leaf behind `t` has its gradient added up on another stream, as it
+// does when an eager graph of it is alive.  The captured backward pass would have to wait for that stream, which ends
+// the process from inside the autograd engine.
+bool adds_up_elsewhere(const at::Tensor& t) {
+  if (!t.requires_grad()) return false;
+  const c10::Stream here = at::cuda::getCurrentCUDAStream(t.get_device()).unwrap();
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  const auto visit = [&](std::shared_ptr<torch::autograd::Node> node) {
+    if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+  };
+  if (t.grad_fn()) visit(t.grad_fn());
+  else visit(torch::autograd::impl::try_get_grad_accumulator(t));
+  while (!todo.empty()) {
+    const auto node = todo.back();
+    todo.pop_back();
+    if (node->num_outputs() == 0) {  // a leaf's
+      const auto stream = node->stream();
+      if (stream && *stream != here) return true;
+    }
+    for (const auto& edge : node->next_edges()) visit(edge.function);
+  }
+  return false;
+}
+
+#define B200_CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
+PyMethodDef kExpertCalls[] = {B200_CALL(rms_norm_fp8), B200_CALL(silu_mul_fp8), B200_CALL(sort_tokens), B200_CALL(unsort_tokens),
+                              B200_CALL(unsort_tokens_backward), {nullptr, nullptr, 0, nullptr}};
+#undef B200_CALL
+
+}  // namespace
+
+void b200::bind_experts(py::module& m) {
+  if (PyModule_AddFunctions(m.ptr(), kExpertCalls) != 0) throw py::error_already_set();
+  m.def("adds_up_elsewhere", &adds_up_elsewhere);
+}

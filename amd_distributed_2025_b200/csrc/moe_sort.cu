@@ -1,0 +1,589 @@
+// Tokens sorted by expert, and their rows back in token order.
+//
+// Entry i = t k + j of the expert ids [T, k] asks for a row of expert e_i.  Rows are packed expert by expert, inside an
+// expert in the order of the entries:
+//   row(i) = offsets[e_i] + #{i' < i : e_i' = e_i},   offsets[e] = #{i : e_i < e}
+// Entries whose id is not in [0, E) have no row (-1); the rows behind offsets[E] are zero.
+//   sort             rows[row(t, j)] = x[t]  (and the same of a scale row)
+//   unsort           out[t] = sum_j w[t, j] rows[row(t, j)]; without weights it is the gradient of sort
+//   unsort backward  grad_rows[row(t, j)] = w[t, j] grad[t],  grad_w[t, j] = <grad[t], rows[row(t, j)]>
+// Sums are fp32, over j upwards, and rounded once; nothing is added by atomics whose order could show in a result (integer
+// counts are).
+//
+// All kernels may start before the previous kernel of the stream has ended: no global memory is touched before
+// grid_dep_wait().
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "moe_common.cuh"
+#include "moe_sort.h"
+#include "per_device.h"
+#include "sm100_ptx.cuh"
+
+namespace b200 {
+
+namespace {
+
+using namespace moe;
+
+// Copies move vectors V, U of them a lane at a time: the widest that rows, their distance and their addresses allow.
+template <typename V> struct Copy { static constexpr int U = sizeof(V) == 16 ? 2 : sizeof(V) == 4 ? 4 : 8; };
+
+struct SortParams {
+  SortTokensArgs a;
+  int32_t pieces;      // of a row; the scales are one more
+  int32_t row_vecs, piece_vecs;
+  int32_t chunks, chunk_tokens, ctas_of_chunk;  // two launches: runs of tokens that are counted by a CTA each
+};
+
+__device__ __forceinline__ int expert_of(const SortTokensArgs& a, int64_t i) {
+  if (a.wide_ids) {
+    const long long e = __ldcg(reinterpret_cast<const long long*>(a.indices) + i);
+    return e >= 0 && e < a.experts ? (int)e : -1;
+  }
+  const int e = __ldcg(reinterpret_cast<const int*>(a.indices) + i);
+  return e >= 0 && e < a.experts ? e : -1;
+}
+
+// counts[0 .. n) in shared memory become exclusive prefix sums; returns their total.  All threads of the CTA.
+__device__ __forceinline__ int exclusive_scan(int32_t* counts, int n, int32_t* warp_sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+  const int each = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int lo = min(n, tid * each), hi = min(n, lo + each);
+  int own = 0;
+  for (int i = lo; i < hi; ++i) own += counts[i];
+  int upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  int run = before + upto - own;
+  for (int i = lo; i < hi; ++i) {
+    const int c = counts[i];
+    counts[i] = run;
+    run += c;
+  }
+  __syncthreads();
+  return total;
+}
+
+// One piece of token t's row (or, behind the last piece, its scales) to its k rows; `row` is lane j's: entry j's row.
+template <typename V>
+__device__ __forceinline__ void copy_piece(const SortParams& p, int t, int piece, int row) {
+  constexpr int U = Copy<V>::U;
+  const int lane = threadIdx.x & 31;
+  const SortTokensArgs& a = p.a;
+  if (piece < p.pieces) {
+    const V* src = reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(a.x) + (int64_t)t * a.x_stride);
+    const int v0 = piece * p.piece_vecs + lane;
+    const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
+    V r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + 32 * u < v1) r[u] = __ldcg(src + v0 + 32 * u);
+    for (int j = 0; j < a.k; ++j) {
+      const int to = __shfl_sync(0xffffffffu, row, j);
+      if (to < 0) continue;
+      V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(a.rows) + (int64_t)to * a.row_bytes);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v0 + 32 * u < v1) dst[v0 + 32 * u] = r[u];
+    }
+  } else {
+    const float* src = a.scale + (int64_t)t * a.scale_stride;
+    for (int c0 = 0; c0 < a.scale_cols; c0 += 32) {
+      const bool in = c0 + lane < a.scale_cols;
+      const float s = in ? __ldcg(src + c0 + lane) : 0.f;
+      for (int j = 0; j < a.k; ++j) {
+        const int to = __shfl_sync(0xffffffffu, row, j);
+        if (to >= 0 && in) a.rows_scale[(int64_t)to * a.scale_cols + c0 + lane] = s;
+      }
+    }
+  }
+}
+
+// Rows [from, to) and their scales are zero: CTA `cta` of `ctas` takes its share.
+template <typename V>
+__device__ __forceinline__ void zero_rows(void* rows, int64_t row_bytes, float* scales, int scale_cols, int64_t from, int64_t to,
+                                          int cta, int ctas) {
+  const V zero = V();
+  for (int64_t r = from + cta; r < to; r += ctas) {
+    V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(rows) + r * row_bytes);
+    for (int v = threadIdx.x; v < (int)(row_bytes / (int64_t)sizeof(V)); v += blockDim.x) dst[v] = zero;
+    if (scales != nullptr)
+      for (int c = threadIdx.x; c < scale_cols; c += blockDim.x) scales[r * scale_cols + c] = 0.f;
+  }
+}
+
+}  // namespace
+
+// One launch: every CTA counts all entries itself, and ranks its own against each other.
+template <typename V>
+__global__ void __launch_bounds__(512) sort_tokens_kernel(const SortParams p) {
+  extern __shared__ int32_t smem[];
+  __shared__ int32_t warp_sums[32];
+  const SortTokensArgs& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x;
+  const int P = p.pieces + (a.scale != nullptr);
+  const int64_t items = (int64_t)a.tokens * P;
+  const int lo = (int)(items * blockIdx.x / gridDim.x), hi = (int)(items * (blockIdx.x + 1) / gridDim.x);
+  const int t0 = lo / P, t1 = hi > lo ? (hi + P - 1) / P : t0;
+  const int i0 = t0 * a.k, i1 = t1 * a.k, n = a.tokens * a.k;
+  int32_t* start = smem;                // entries of all of an expert, then the first row of each
+  int32_t* before = start + a.experts;  // own entries and earlier ones
+  int32_t* ids = before + a.experts;    // expert of each own entry, then its row
+  for (int e = tid; e < 2 * a.experts; e += threads) smem[e] = 0;
+  __syncthreads();
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  for (int i = tid; i < n; i += threads) {
+    const int e = expert_of(a, i);
+    if (e >= 0) {
+      atomicAdd(start + e, 1);
+      if (i < i1) atomicAdd(before + e, 1);
+    }
+    if (i >= i0 && i < i1) ids[i - i0] = e;
+  }
+  __syncthreads();
+  const int total = exclusive_scan(start, a.experts, warp_sums);
+  // an entry's rank is the count up to the CTA's end less the own entries of its expert from it on
+  for (int j0 = tid - lane; j0 < i1 - i0; j0 += threads) {
+    const int j = j0 + lane;
+    const int e = j < i1 - i0 ? ids[j] : -1;
+    int from_here = __popc(__match_any_sync(0xffffffffu, e) & (0xffffffffu << lane));
+    for (int q = j0 + 32; q < i1 - i0; ++q) from_here += ids[q] == e;
+    if (j < i1 - i0) ids[i1 - i0 + j] = e < 0 ? -1 : start[e] + before[e] - from_here;
+  }
+  __syncthreads();
+  const int32_t* rows = ids + (i1 - i0);
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < a.experts; e += threads) a.offsets[e] = start[e];
+    if (tid == 0) a.offsets[a.experts] = total;
+  }
+  for (int item = lo + (tid >> 5); item < hi; item += threads >> 5) {
+    const int t = item / P, piece = item - t * P;
+    const int row = lane < a.k ? rows[t * a.k - i0 + lane] : -1;
+    if (piece == 0 && lane < a.k) a.row_of[t * a.k + lane] = row;
+    copy_piece<V>(p, t, piece, row);
+  }
+  zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, n, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// Two launches, the first: a CTA counts a run of tokens' entries by expert, and ranks them inside the run.  Warps have runs
+// of their own inside it, so that order needs no other means than a prefix over warps.
+// work: [chunk][expert] counts, then a rank for each entry.
+__global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
+  extern __shared__ int32_t smem[];  // [warp][expert]
+  const SortTokensArgs& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+  const int c = blockIdx.x;
+  for (int e = tid; e < warps * a.experts; e += blockDim.x) smem[e] = 0;
+  __syncthreads();
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  const int i0 = c * p.chunk_tokens * a.k, i1 = min(a.tokens, (c + 1) * p.chunk_tokens) * a.k;
+  const int each = ((i1 - i0 + warps - 1) / warps + 31) & ~31;
+  const int w0 = min(i1, i0 + warp * each), w1 = min(i1, w0 + each);
+  int32_t* own = smem + warp * a.experts;
+  int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
+  for (int i = w0 + lane; i - lane < w1; i += 32) {
+    const int e = i < w1 ? expert_of(a, i) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    int rank = 0;
+    if (e >= 0) rank = own[e] + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (e >= 0 && (same >> lane) == 1u) own[e] = rank + 1;  // (the last of them)
+    __syncwarp();
+    if (i < w1) ranks[i] = rank;
+  }
+  __syncthreads();
+  for (int e = tid; e < a.experts; e += blockDim.x) {
+    int run = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int n = smem[w * a.experts + e];
+      smem[w * a.experts + e] = run;
+      run += n;
+    }
+    a.work[(int64_t)c * a.experts + e] = run;
+  }
+  __syncthreads();
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const int e = expert_of(a, i);
+    if (e >= 0) ranks[i] += own[e];
+  }
+}
+
+// The second: a CTA adds up the runs' counts, and copies its share of one run's rows.
+template <typename V>
+__global__ void __launch_bounds__(512) sort_scatter_kernel(const SortParams p) {
+  extern __shared__ int32_t smem[];
+  __shared__ int32_t warp_sums[32];
+  const SortTokensArgs& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x, warps = threads >> 5;
+  const int c = (int)blockIdx.x / p.ctas_of_chunk, g = (int)blockIdx.x - c * p.ctas_of_chunk;
+  int32_t* start = smem;
+  int32_t* base = start + a.experts;
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  for (int e = tid; e < a.experts; e += threads) {
+    int all = 0, earlier = 0;
+    for (int q = 0; q < p.chunks; ++q) {
+      const int n = __ldcg(a.work + (int64_t)q * a.experts + e);
+      all += n;
+      earlier += q < c ? n : 0;
+    }
+    start[e] = all;
+    base[e] = earlier;
+  }
+  __syncthreads();
+  const int total = exclusive_scan(start, a.experts, warp_sums);
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < a.experts; e += threads) a.offsets[e] = start[e];
+    if (tid == 0) a.offsets[a.experts] = total;
+  }
+  const int P = p.pieces + (a.scale != nullptr);
+  const int t0 = c * p.chunk_tokens, t1 = min(a.tokens, t0 + p.chunk_tokens);
+  const int64_t items = (int64_t)(t1 - t0) * P;
+  const int64_t lo = items * g / p.ctas_of_chunk, hi = items * (g + 1) / p.ctas_of_chunk;
+  const int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
+  for (int64_t item = lo + (tid >> 5); item < hi; item += warps) {
+    const int t = t0 + (int)(item / P), piece = (int)(item % P);
+    int row = -1;
+    if (lane < a.k) {
+      const int64_t i = (int64_t)t * a.k + lane;
+      const int e = expert_of(a, i);
+      if (e >= 0) row = start[e] + base[e] + __ldcg(ranks + i);
+      if (piece == 0) a.row_of[i] = row;
+    }
+    copy_piece<V>(p, t, piece, row);
+  }
+  zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, (int64_t)a.tokens * a.k, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// ---------------------------------------------------------------------------------------
+// back to the tokens
+// ---------------------------------------------------------------------------------------
+namespace {
+
+// What a lane takes of a row at once: sixteen bytes, or one element where rows are not whole aligned 16-byte vectors.
+template <typename T, bool VEC> struct Bit;
+template <typename T> struct Bit<T, true> {
+  static constexpr int N = Vec16<T>::N;
+  using Raw = int4;
+  static __device__ __forceinline__ void fma(float* acc, const Raw& r, float w) { fma_vec<T>(acc, r, w); }
+  static __device__ __forceinline__ Raw pack(const float* acc) { return pack_vec<T>(acc); }
+};
+template <typename T> struct Bit<T, false> {
+  static constexpr int N = 1;
+  using Raw = T;
+  static __device__ __forceinline__ void fma(float* acc, const Raw& r, float w) { acc[0] = fmaf(to_f32(r), w, acc[0]); }
+  static __device__ __forceinline__ Raw pack(const float* acc) { return from_f32<T>(acc[0]); }
+};
+
+struct UnsortParams {
+  UnsortTokensArgs a;
+  int32_t row_vecs, pieces, piece_vecs;
+};
+struct UnsortBackwardParams {
+  UnsortBackwardArgs a;
+  int32_t row_vecs;
+};
+
+}  // namespace
+
+// A warp takes a piece of a token's row: U vectors a lane of KB rows at a time.
+template <typename T, bool VEC, int KB>
+__global__ void __launch_bounds__(256) unsort_tokens_kernel(const UnsortParams p) {
+  using B = Bit<T, VEC>;
+  using Raw = typename B::Raw;
+  constexpr int U = VEC ? 2 : 4;
+  const UnsortTokensArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = ((int64_t)gridDim.x * blockDim.x) >> 5;
+  const int64_t items = (int64_t)a.tokens * p.pieces;
+  const uint8_t* rows = reinterpret_cast<const uint8_t*>(a.rows);
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  for (int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; item < items; item += warps) {
+    const int t = (int)(item / p.pieces), piece = (int)(item % p.pieces);
+    int row = -1;
+    float w = 1.f;
+    if (lane < a.k) {
+      row = __ldcg(a.row_of + (int64_t)t * a.k + lane);
+      if (a.weights != nullptr) w = __ldcg(a.weights + (int64_t)t * a.k + lane);
+      if (row >= a.num_rows) row = -1;
+    }
+    Raw* out = reinterpret_cast<Raw*>(reinterpret_cast<T*>(a.out) + (int64_t)t * a.hidden);
+    const int v0 = piece * p.piece_vecs, v1 = min(p.row_vecs, v0 + p.piece_vecs);
+    for (int vb = v0; vb < v1; vb += 32 * U) {
+      float acc[U][B::N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < B::N; ++e) acc[u][e] = 0.f;
+      for (int kb = 0; kb < a.k; kb += KB) {
+        // all loads leave before the first is used: a lane past the end, or an entry without a row, reads a valid place
+        // (its own batch's last vector, row 0) and drops the value
+        Raw r[KB][U];
+#pragma unroll
+        for (int q = 0; q < KB; ++q) {
+          const int from = max(__shfl_sync(0xffffffffu, row, min(kb + q, a.k - 1)), 0);
+          const Raw* src = reinterpret_cast<const Raw*>(rows + (int64_t)from * a.rows_stride);
+#pragma unroll
+          for (int u = 0; u < U; ++u) r[q][u] = __ldcg(src + min(vb + lane + 32 * u, v1 - 1));
+        }
+#pragma unroll
+        for (int q = 0; q < KB; ++q) {
+          const int from = kb + q < a.k ? __shfl_sync(0xffffffffu, row, kb + q) : -1;
+          const float wq = __shfl_sync(0xffffffffu, w, (kb + q) & 31);
+          if (from < 0) continue;
+#pragma unroll
+          for (int u = 0; u < U; ++u) B::fma(acc[u], r[q][u], wq);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (vb + lane + 32 * u < v1) out[vb + lane + 32 * u] = B::pack(acc[u]);
+    }
+  }
+}
+
+// A CTA takes a token.  DOT: the weights' gradient is wanted, so the rows are read.
+template <typename T, bool VEC, bool DOT>
+__global__ void __launch_bounds__(256) unsort_tokens_backward_kernel(const UnsortBackwardParams p) {
+  using B = Bit<T, VEC>;
+  using Raw = typename B::Raw;
+  constexpr int KB = 4;
+  __shared__ float parts[8][kSortMaxTopk];
+  const UnsortBackwardArgs& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+  const int64_t row_bytes = (int64_t)a.hidden * (int64_t)sizeof(T);
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    int row = -1;
+    float w = 1.f;
+    if (lane < a.k) {
+      row = __ldcg(a.row_of + (int64_t)t * a.k + lane);
+      if (a.weights != nullptr) w = __ldcg(a.weights + (int64_t)t * a.k + lane);
+      if (row >= a.num_rows) row = -1;
+    }
+    const Raw* grad = reinterpret_cast<const Raw*>(reinterpret_cast<const uint8_t*>(a.grad) + (int64_t)t * a.grad_stride);
+    for (int kb = 0; kb < a.k; kb += KB) {
+      float dot[KB];
+      int from[KB];
+      float wq[KB];
+#pragma unroll
+      for (int q = 0; q < KB; ++q) {
+        dot[q] = 0.f;
+        from[q] = __shfl_sync(0xffffffffu, row, (kb + q) & 31);
+        if (kb + q >= a.k) from[q] = -1;
+        wq[q] = __shfl_sync(0xffffffffu, w, (kb + q) & 31);
+      }
+      for (int v = tid; v < p.row_vecs; v += blockDim.x) {
+        const Raw g = grad[v];
+        Raw y[KB];
+        if (DOT) {
+#pragma unroll
+          for (int q = 0; q < KB; ++q)
+            y[q] = __ldcg(reinterpret_cast<const Raw*>(reinterpret_cast<const uint8_t*>(a.rows) +
+                                                       (int64_t)max(from[q], 0) * a.rows_stride) + v);
+        }
+        float gf[B::N];
+#pragma unroll
+        for (int e = 0; e < B::N; ++e) gf[e] = 0.f;
+        B::fma(gf, g, 1.f);
+#pragma unroll
+        for (int q = 0; q < KB; ++q) {
+          if (from[q] < 0) continue;
+          if (DOT) {
+            float yf[B::N];
+#pragma unroll
+            for (int e = 0; e < B::N; ++e) yf[e] = 0.f;
+            B::fma(yf, y[q], 1.f);
+#pragma unroll
+            for (int e = 0; e < B::N; ++e) dot[q] = fmaf(gf[e], yf[e], dot[q]);
+          }
+          if (a.grad_rows != nullptr) {
+            float d[B::N];
+#pragma unroll
+            for (int e = 0; e < B::N; ++e) d[e] = gf[e] * wq[q];
+            reinterpret_cast<Raw*>(reinterpret_cast<uint8_t*>(a.grad_rows) + (int64_t)from[q] * row_bytes)[v] = B::pack(d);
+          }
+        }
+      }
+      if (DOT) {
+#pragma unroll
+        for (int q = 0; q < KB; ++q) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], o);
+          if (lane == 0 && kb + q < a.k) parts[warp][kb + q] = dot[q];
+        }
+      }
+    }
+    if (DOT) {
+      __syncthreads();
+      if (tid < a.k) {
+        float sum = 0.f;
+        for (int i = 0; i < warps; ++i) sum += parts[i][tid];
+        a.grad_weights[(int64_t)t * a.k + tid] = sum;
+      }
+      __syncthreads();
+    }
+  }
+  if (a.grad_rows != nullptr) {
+    const int64_t end = max(0, __ldcg(a.end));
+    zero_rows<Raw>(a.grad_rows, row_bytes, nullptr, 0, end, a.num_rows, (int)blockIdx.x, (int)gridDim.x);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------
+namespace {
+
+constexpr int64_t kOneLaunchEntries = 16384;
+constexpr int kMaxChunks = 64;
+constexpr int kCountSmem = 160 * 1024;  // of the counting kernel: a count of every expert for each warp
+
+int sort_chunks(int64_t tokens, int k) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxChunks, tokens * k / 2048));
+}
+
+template <typename V>
+cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
+  const SortTokensArgs& a = p.a;
+  p.row_vecs = (int)(a.row_bytes / (int64_t)sizeof(V));
+  p.piece_vecs = 32 * Copy<V>::U;
+  p.pieces = std::max(1, (p.row_vecs + p.piece_vecs - 1) / p.piece_vecs);
+  const int64_t items = (int64_t)a.tokens * (p.pieces + (a.scale != nullptr));
+  if (a.work == nullptr) {
+    if (items > INT32_MAX) return cudaErrorInvalidValue;
+    const int threads = 512;
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + 15) / 16, 2 * (int64_t)sms));
+    const int P = p.pieces + (a.scale != nullptr);
+    const int64_t own = ((items + grid - 1) / grid + 2 * P - 2) / P * a.k;  // entries of the tokens that a CTA touches, at most
+    const size_t smem = (2 * (size_t)a.experts + 2 * (size_t)own) * sizeof(int32_t);
+    static OncePerDevice once;
+    const cudaError_t opted = once([] { return opt_in(sort_tokens_kernel<V>, kCountSmem, false); });
+    if (opted != cudaSuccess) return opted;
+    if (smem > kCountSmem) return cudaErrorInvalidValue;
+    return ptx::launch_dependent(sort_tokens_kernel<V>, grid, threads, smem, stream, p);
+  }
+  p.chunks = sort_chunks(a.tokens, a.k);
+  p.chunk_tokens = (a.tokens + p.chunks - 1) / p.chunks;
+  p.chunks = (a.tokens + p.chunk_tokens - 1) / p.chunk_tokens;
+  static OncePerDevice once;
+  const cudaError_t opted = once([] {
+    const cudaError_t e = opt_in(sort_count_kernel, kCountSmem, false);
+    return e != cudaSuccess ? e : opt_in(sort_scatter_kernel<V>, 2 * kSortMaxExperts * (int)sizeof(int32_t), false);
+  });
+  if (opted != cudaSuccess) return opted;
+  const int warps = std::max(1, std::min(32, kCountSmem / (a.experts * (int)sizeof(int32_t))));
+  cudaError_t e = ptx::launch_dependent(sort_count_kernel, p.chunks, 32 * warps, (size_t)warps * a.experts * sizeof(int32_t),
+                                        stream, p);
+  if (e != cudaSuccess) return e;
+  p.ctas_of_chunk = std::max(1, (2 * sms + p.chunks - 1) / p.chunks);
+  return ptx::launch_dependent(sort_scatter_kernel<V>, p.chunks * p.ctas_of_chunk, 512, 2 * (size_t)a.experts * sizeof(int32_t),
+                               stream, p);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, bool VEC>
+cudaError_t unsort_typed(const UnsortTokensArgs& a, int sms, cudaStream_t stream) {
+  UnsortParams p;
+  p.a = a;
+  p.row_vecs = a.hidden / Bit<T, VEC>::N;
+  p.piece_vecs = VEC ? 64 : 128;
+  p.pieces = (p.row_vecs + p.piece_vecs - 1) / p.piece_vecs;
+  const int64_t items = (int64_t)a.tokens * p.pieces;
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, 4 * (int64_t)sms));
+  switch (a.k) {
+    case 1: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 1>, grid, 256, 0, stream, p);
+    case 2: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 2>, grid, 256, 0, stream, p);
+    default: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 4>, grid, 256, 0, stream, p);
+  }
+}
+
+template <typename T>
+cudaError_t unsort_vec(const UnsortTokensArgs& a, int sms, cudaStream_t stream) {
+  const bool vec = a.hidden % Vec16<T>::N == 0 && a.rows_stride % 16 == 0 && aligned16(a.rows) && aligned16(a.out);
+  return vec ? unsort_typed<T, true>(a, sms, stream) : unsort_typed<T, false>(a, sms, stream);
+}
+
+template <typename T, bool VEC>
+cudaError_t backward_typed(const UnsortBackwardArgs& a, int sms, cudaStream_t stream) {
+  UnsortBackwardParams p;
+  p.a = a;
+  p.row_vecs = a.hidden / Bit<T, VEC>::N;
+  const int threads = std::max(32, std::min(256, (p.row_vecs / 2 + 31) / 32 * 32));
+  const int grid = (int)std::min<int64_t>(std::max(a.tokens, 1), 1 << 30);
+  return a.grad_weights != nullptr
+             ? ptx::launch_dependent(unsort_tokens_backward_kernel<T, VEC, true>, grid, threads, 0, stream, p)
+             : ptx::launch_dependent(unsort_tokens_backward_kernel<T, VEC, false>, grid, threads, 0, stream, p);
+}
+
+template <typename T>
+cudaError_t backward_vec(const UnsortBackwardArgs& a, int sms, cudaStream_t stream) {
+  const bool vec = a.hidden % Vec16<T>::N == 0 && a.grad_stride % 16 == 0 && a.rows_stride % 16 == 0 && aligned16(a.grad) &&
+                   aligned16(a.rows) && aligned16(a.grad_rows);
+  return vec ? backward_typed<T, true>(a, sms, stream) : backward_typed<T, false>(a, sms, stream);
+}
+
+}  // namespace
+
+int64_t sort_tokens_work(int64_t tokens, int k, int experts) {
+  if (tokens * k <= kOneLaunchEntries) return 0;
+  return (int64_t)sort_chunks(tokens, k) * experts + tokens * k;
+}
+
+cudaError_t launch_sort_tokens(const SortTokensArgs& a, int sms, cudaStream_t stream) {
+  if (a.tokens < 0 || a.k < 1 || a.k > kSortMaxTopk || a.experts < 1 || a.experts > kSortMaxExperts ||
+      (int64_t)a.tokens * a.k > INT32_MAX)
+    return cudaErrorInvalidValue;
+  SortParams p = {};
+  p.a = a;
+  const uint64_t bits = (uint64_t)a.row_bytes | (uint64_t)a.x_stride | reinterpret_cast<uintptr_t>(a.x) |
+                        reinterpret_cast<uintptr_t>(a.rows);
+  if (bits % 16 == 0) return sort_typed<int4>(p, sms, stream);
+  if (bits % 4 == 0) return sort_typed<int>(p, sms, stream);
+  if (bits % 2 == 0) return sort_typed<short>(p, sms, stream);
+  return sort_typed<signed char>(p, sms, stream);
+}
+
+cudaError_t launch_unsort_tokens(const UnsortTokensArgs& a, int sms, cudaStream_t stream) {
+  if (a.tokens < 0 || a.k < 1 || a.k > kSortMaxTopk || a.hidden < 1) return cudaErrorInvalidValue;
+  if (a.tokens == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case 0: return unsort_vec<__half>(a, sms, stream);
+    case 1: return unsort_vec<__nv_bfloat16>(a, sms, stream);
+    case 2: return unsort_vec<float>(a, sms, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_unsort_tokens_backward(const UnsortBackwardArgs& a, int sms, cudaStream_t stream) {
+  if (a.tokens < 0 || a.k < 1 || a.k > kSortMaxTopk || a.hidden < 1) return cudaErrorInvalidValue;
+  if (a.tokens == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case 0: return backward_vec<__half>(a, sms, stream);
+    case 1: return backward_vec<__nv_bfloat16>(a, sms, stream);
+    case 2: return backward_vec<float>(a, sms, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace b200

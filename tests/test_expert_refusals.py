@@ -1,0 +1,98 @@
+"""Calls of the operators around a GPU's experts that are refused before anything is launched (no GPU needed)."""
+import pytest
+import torch
+
+from amd_distributed_2025_b200.ops import fp8_rows, moe_sort
+from amd_distributed_2025_b200.ops.moe_sort import ExpertOrder
+
+F = torch.zeros
+
+
+def _refused(match, call):
+    with pytest.raises((RuntimeError, ValueError, TypeError), match=match):
+        call()
+
+
+def test_rms_norm_fp8_refusals():
+    x, w = F(4, 256), F(256)
+    f = fp8_rows.rms_norm_fp8
+    _refused("matrix", lambda: f(F(256), w))
+    _refused("matrix", lambda: f(F(2, 2, 256), w))
+    _refused("unsupported dtype", lambda: f(x.double(), w.double()))
+    _refused("unsupported dtype", lambda: f(x.to(torch.float8_e4m3fn), w))
+    _refused("weight must be a vector", lambda: f(x, F(255)))
+    _refused("weight must be a vector", lambda: f(x, F(1, 256)))
+    _refused("weight must have x's type", lambda: f(x, w.half()))
+    _refused("columns", lambda: f(F(2, 0), F(0)))
+    _refused("columns", lambda: f(F(1, 32769), F(32769)))
+    _refused("eps", lambda: f(x, w, -1.0))
+    _refused("eps", lambda: f(x, w, float("nan")))
+    _refused("residual must", lambda: f(x, w, residual=F(4, 255)))
+    _refused("residual must", lambda: f(x, w, residual=x.half()))
+    _refused("there is no residual", lambda: f(x, w, total_out=x))
+    _refused("total_out must have x's", lambda: f(x, w, residual=x, total_out=F(3, 256)))
+    _refused("total_out must have contiguous rows", lambda: f(x, w, residual=x, total_out=F(256, 4).t()))
+    _refused("total_out must have contiguous rows", lambda: f(x, w, residual=x, total_out=F(1, 256).expand(4, 256)))
+    _refused("no_grad", lambda: f(x.clone().requires_grad_(), w))
+    _refused("no_grad", lambda: f(x, w.clone().requires_grad_()))
+    _refused("no_grad", lambda: f(x, w, residual=x.clone().requires_grad_()))
+    _refused("CUDA", lambda: f(x, w))
+    with torch.no_grad():  # a parameter is fine there
+        _refused("CUDA", lambda: f(x, w.clone().requires_grad_()))
+    _refused("expected a torch.Tensor", lambda: f(None, w))
+
+
+def test_silu_mul_fp8_refusals():
+    f = fp8_rows.silu_mul_fp8
+    _refused("matrix", lambda: f(F(256)))
+    _refused("even number", lambda: f(F(4, 255)))
+    _refused("even number", lambda: f(F(4, 0)))
+    _refused("unsupported dtype", lambda: f(F(4, 256, dtype=torch.int32)))
+    _refused("no_grad", lambda: f(F(4, 256).requires_grad_()))
+    _refused("CUDA", lambda: f(F(4, 256)))
+
+
+def test_sort_tokens_refusals():
+    x, ids = F(4, 64), F(4, 2, dtype=torch.int32)
+    f = moe_sort.sort_tokens
+    _refused("x must be a matrix", lambda: f(F(4), ids, 8))
+    _refused("x must be a matrix", lambda: f(F(4, 0), ids, 8))
+    _refused("unsupported dtype", lambda: f(x.double(), ids, 8))
+    _refused("indices must be", lambda: f(x, ids[:3], 8))
+    _refused("indices must be", lambda: f(x, ids[0], 8))
+    _refused("int32 or int64", lambda: f(x, ids.to(torch.int16), 8))
+    _refused("int32 or int64", lambda: f(x, ids.float(), 8))
+    _refused("1 to 32 experts", lambda: f(x, F(4, 0, dtype=torch.int32), 8))
+    _refused("1 to 32 experts", lambda: f(x, F(4, 33, dtype=torch.int32), 64))
+    _refused("num_experts", lambda: f(x, ids, 0))
+    _refused("num_experts", lambda: f(x, ids, 8193))
+    _refused("2\\^30", lambda: f(F(1, 1).expand(1 << 29, 1), F(1, 1, dtype=torch.int32).expand(1 << 29, 4), 8))
+    _refused("scale must be", lambda: f(x, ids, 8, scale=F(3, 1)))
+    _refused("scale must be", lambda: f(x, ids, 8, scale=F(4, 1).half()))
+    _refused("no gradient", lambda: f(x.clone().requires_grad_(), ids, 8, scale=F(4, 1)))
+    _refused("CUDA", lambda: f(x, ids, 8))
+
+
+def test_unsort_tokens_refusals():
+    order = ExpertOrder(F(9, dtype=torch.int32), F(4, 2, dtype=torch.int32))
+    rows, w = F(8, 64), F(4, 2)
+    f = moe_sort.unsort_tokens
+    _refused("rows must be a matrix", lambda: f(F(8), order, w))
+    _refused("unsupported dtype", lambda: f(rows.to(torch.float8_e4m3fn), order, w))
+    _refused("a row for each", lambda: f(F(7, 64), order, w))
+    _refused("a row for each", lambda: f(F(9, 64), order, w))
+    _refused("weights must be", lambda: f(rows, order, F(4, 3)))
+    _refused("weights must be", lambda: f(rows, order, F(8)))
+    _refused("row_of must be", lambda: f(rows, ExpertOrder(order.offsets, order.row_of.long()), w))
+    _refused("row_of must be", lambda: f(rows, ExpertOrder(order.offsets, order.row_of[0]), w))
+    _refused("CUDA", lambda: f(rows, order, w))
+    b = moe_sort.unsort_tokens_backward
+    grad = F(4, 64)
+    _refused("gradient must be", lambda: b(F(4, 63), rows, order, w))
+    _refused("gradient must be", lambda: b(grad.half(), rows, order, w))
+    _refused("a row for each", lambda: b(grad, F(9, 64), order, w))
+    _refused("offsets must be", lambda: b(grad, rows, ExpertOrder(order.offsets.long(), order.row_of), w))
+    _refused("offsets must be", lambda: b(grad, rows, ExpertOrder(order.offsets[:1], order.row_of), w))
+    _refused("weights must be", lambda: b(grad, rows, order, F(4, 3)))
+    _refused("CUDA", lambda: b(grad, rows, order, w))
+    _refused("a row for each", lambda: moe_sort.sort_tokens_backward(F(7, 64), order))

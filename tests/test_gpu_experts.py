@@ -1,0 +1,554 @@
+"""The operators around a GPU's experts against plain implementations in 64 bits.
+
+Tolerances count roundings: half a step of a type (u = finfo.eps / 2) for each output that is rounded to it, 2^-24 for each
+fp32 operation on the longest chain behind it."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(*shape, dtype=torch.float32, seed=0):
+    return torch.randn(*shape, device="cuda", generator=_gen(seed)).to(dtype)
+
+
+def _close(got, want, bound, what=""):
+    """|got - want| <= bound everywhere (a bound of the values' shape, or a number)."""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape
+    assert torch.equal(got.isnan(), want.isnan()), what
+    off = (got - want).abs() - bound
+    worst = off.nan_to_num(nan=-1.0).max().item() if off.numel() else -1.0
+    assert worst <= 0, f"{what}: {worst:.3g} over the bound"
+
+
+# --------------------------------------------------------------------------------------
+# rows with block scales
+# --------------------------------------------------------------------------------------
+
+def _e4m3(v):
+    """Nearest e4m3 value of |v| <= 448, ties to even, in 64 bits."""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6)))) / 8
+    return torch.round(v / step) * step
+
+
+def _check_quantised(q, scale, y, rel):
+    """q and scale against y [rows, cols] in 64 bits, which the kernel knows to within a factor of 1 +- rel."""
+    rows, cols = y.shape
+    blocks = -(-cols // 128)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == (rows, cols) and q.is_contiguous()
+    assert scale.dtype == torch.float32 and scale.shape == (rows, blocks) and scale.is_contiguous()
+    padded = torch.nn.functional.pad(y, (0, blocks * 128 - cols)).view(rows, blocks, 128)
+    want = padded.abs().amax(2).clamp(min=1e-30) / 448
+    _close(scale, want, (rel + 2 * U32) * want, "scale")
+    v = (padded / want[:, :, None]).view(rows, -1)[:, :cols]
+    # the kernel's quotient is v to within twice that and the roundings of reciprocal, product and scale
+    slack = 2 * rel + 6 * U32
+    low, high = _e4m3((v.abs() * (1 - slack))), _e4m3((v.abs() * (1 + slack)).clamp(max=448))
+    got = q.double()
+    assert bool(((got.abs() >= low) & (got.abs() <= high)).all())
+    assert bool((got * v >= 0).all())
+
+
+def _norm_rel(cols):
+    # sum of squares: a lane's chain of cols / 32 terms at most (cols / 512 from 1024 columns on), ten steps to add up the
+    # lanes; the root halves that; the sum of x and residual, the mean, the reciprocal root (two steps), two products
+    return (max(cols / 512, min(cols, 2048) / 32) / 2 + 16) * U32
+
+
+def _norm_case(rows, cols, dtype, residual, normed, weight_dtype=None, seed=1):
+    x = _randn(rows, cols, dtype=dtype, seed=seed)
+    w = (1 + 0.2 * _randn(cols, seed=seed + 1)).to(weight_dtype or dtype)
+    r = (3 * _randn(rows, cols, seed=seed + 2)).to(dtype) if residual else None
+    return x, w, r, normed
+
+
+def _check_norm(x, w, r, got, eps=1e-6):
+    rows, cols = x.shape
+    h = x.double() + (r.double() if r is not None else 0)
+    # y * (1 + rel): fp32 addition is off by U32 |h|
+    y = h / torch.sqrt(h.square().mean(1, keepdim=True) + eps) * w.double()
+    rel = _norm_rel(cols)
+    _check_quantised(got.q, got.scale, y, rel)
+    if r is None:
+        assert got.total is None
+    else:
+        assert got.total.dtype == x.dtype
+        _close(got.total, h, (_u(x.dtype) + U32) * h.abs() + 2.0 ** -25, "total")
+    if got.normed is not None:
+        assert got.normed.dtype == x.dtype
+        _close(got.normed, y, (_u(x.dtype) + rel) * y.abs() + 2.0 ** -25, "normed")  # (2^-25: half of fp16's least step)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 8), (9, 127), (8, 128), (17, 129), (4, 513), (33, 1000), (2, 1024),
+                                       (3, 1032), (1, 2880), (7, 4097), (130, 4096), (1, 7168), (3, 8200), (2, 16392), (2, 32768),
+                                       (1, 32767)])
+def test_rms_norm_fp8(rows, cols, dtype):
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    for residual, normed in ((False, False), (True, True)):
+        x, w, r, normed = _norm_case(rows, cols, dtype, residual, normed)
+        got = rms_norm_fp8(x, w, 1e-6, residual=r, normed=normed)
+        assert (got.normed is not None) == normed
+        _check_norm(x, w, r, got)
+
+
+def test_rms_norm_fp8_weight_in_fp32_strides_and_alignment():
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    x, w, r, _ = _norm_case(6, 512, torch.bfloat16, True, True, torch.float32)
+    _check_norm(x, w, r, rms_norm_fp8(x, w, residual=r, normed=True))
+    wide, other = _randn(6, 2000, dtype=torch.float16, seed=3), _randn(6, 1001, dtype=torch.float16, seed=4)
+    w16 = w.half()
+    for lo in (0, 8, 1, 4):  # columns of a wider matrix: whole vectors, and not
+        x, r = wide[:, lo:lo + 512], other[:, lo:lo + 512]
+        _check_norm(x, w16, r, rms_norm_fp8(x, w16, residual=r))
+    x = _randn(512, 6, dtype=torch.float16, seed=5).t()  # rows that are not contiguous
+    _check_norm(x, w16, None, rms_norm_fp8(x, w16))
+    x = _randn(1, 512, dtype=torch.float16, seed=6).expand(6, 512)  # the same row six times
+    _check_norm(x, w16, None, rms_norm_fp8(x, w16, normed=True))
+    shifted = torch.empty(513, dtype=torch.float16, device="cuda")[1:].copy_(w16)
+    _check_norm(wide[:, :512], shifted, None, rms_norm_fp8(wide[:, :512], shifted))
+
+
+@pytest.mark.parametrize("cols", [1024, 1500, 4100])
+def test_rms_norm_fp8_total_in_place(cols):
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    x, w, r, _ = _norm_case(40, cols, torch.bfloat16, True, False)
+    want = rms_norm_fp8(x, w, residual=r)
+    kept = r.clone()
+    got = rms_norm_fp8(x, w, residual=kept, total_out=kept)
+    assert got.total is kept or got.total.data_ptr() == kept.data_ptr()
+    assert torch.equal(kept, want.total) and torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8))
+    kept = x.clone()
+    got = rms_norm_fp8(kept, w, residual=r, total_out=kept)
+    assert torch.equal(kept, want.total) and torch.equal(got.scale, want.scale)
+    room = torch.full((40, cols + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    rms_norm_fp8(x, w, residual=r, total_out=room[:, 8:8 + cols])
+    assert torch.equal(room[:, 8:8 + cols], want.total)
+    assert bool((room[:, :8] == 7).all()) and bool((room[:, 8 + cols:] == 7).all())
+    both = torch.zeros(41, cols, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap|memory location"):
+        rms_norm_fp8(both[:40], w, residual=r, total_out=both[1:])
+
+
+def test_rms_norm_fp8_zeros_infinities_and_nan():
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    x = _randn(6, 300, dtype=torch.bfloat16, seed=8)
+    w = torch.ones(300, dtype=torch.bfloat16, device="cuda")
+    x[0] = 0
+    x[1, 128:] = 0
+    x[2, 5] = float("nan")
+    x[3, 200] = float("inf")
+    x[4, :] = 1e-30
+    got = rms_norm_fp8(x, w)
+    assert bool((got.q[0].float() == 0).all()) and bool((got.q[1, 128:].float() == 0).all())
+    assert bool(got.scale[0].isfinite().all()) and bool((got.scale[0] > 0).all())
+    assert bool(got.q[2].float().isnan().all()) and bool(got.scale[2].isnan().all())  # the whole row's norm is NaN
+    # one infinity: its own block is NaN, and the others are zero (everything over infinity)
+    assert bool(got.q[3, 128:256].float().isnan().all()) and bool((got.q[3, :128].float() == 0).all())
+    assert bool(got.q[4].float().isfinite().all())
+    _check_norm(x[5:], w, None, rms_norm_fp8(x[5:], w))
+    assert torch.equal(got.q[5].view(torch.uint8), rms_norm_fp8(x[5:], w).q[0].view(torch.uint8))
+    empty = rms_norm_fp8(x[:0], w, residual=x[:0], normed=True)
+    assert empty.q.shape == (0, 300) and empty.scale.shape == (0, 3) and empty.total.shape == empty.normed.shape == (0, 300)
+
+
+def _check_silu(x, got):
+    cols = x.shape[1] // 2
+    g, u = x[:, :cols].double(), x[:, cols:].double()
+    y = g / (1 + torch.exp(-g)) * u
+    # exp to two steps, and a step for each unit of the exponent that is rounded before it; sum, quotient (two steps), product
+    rel = (x[:, :cols].abs().max().double().item() * 1.5 + 8) * U32 if x.numel() else 0.0
+    _check_quantised(got[0], got[1], y, rel)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 8), (3, 127), (9, 128), (2, 130), (33, 360), (7, 1000), (130, 2048), (1, 2880),
+                                       (3, 8192), (2, 8191)])
+def test_silu_mul_fp8(rows, cols, dtype):
+    from amd_distributed_2025_b200.ops.fp8_rows import silu_mul_fp8
+
+    x = _randn(rows, 2 * cols, dtype=dtype, seed=rows + cols) * 2
+    _check_silu(x, silu_mul_fp8(x))
+
+
+def test_silu_mul_fp8_strides_and_special_values():
+    from amd_distributed_2025_b200.ops.fp8_rows import silu_mul_fp8
+
+    wide = _randn(9, 3000, dtype=torch.bfloat16, seed=4)
+    for lo in (0, 8, 3):
+        x = wide[:, lo:lo + 1024]
+        _check_silu(x, silu_mul_fp8(x))
+    x = _randn(1024, 5, dtype=torch.float16, seed=4).t()
+    _check_silu(x, silu_mul_fp8(x))
+    x = torch.zeros(4, 512, device="cuda")
+    x[:, 256:] = 1.0
+    x[0, 3] = float("nan")
+    x[1, :256] = -200.0  # exp overflows: the gate is -0, not NaN
+    x[2, 7] = float("inf")
+    q, scale = silu_mul_fp8(x)
+    assert bool(q[0, :128].float().isnan().all()) and bool((q[0, 128:].float() == 0).all())
+    assert bool((q[1].float() == 0).all())
+    assert bool(scale[2, 0].isinf()) and bool(q[2, 7].float().isnan()) and bool((q[2, 128:].float() == 0).all())
+    assert bool((q[3].float() == 0).all())
+    q, scale = silu_mul_fp8(x[:0])
+    assert q.shape == (0, 256) and scale.shape == (0, 2)
+
+
+# --------------------------------------------------------------------------------------
+# tokens sorted by expert
+# --------------------------------------------------------------------------------------
+
+def _ids(tokens, k, experts, seed, kind="uniform", dtype=torch.int32):
+    g = _gen(seed)
+    if kind == "uniform":
+        ids = torch.randint(0, experts, (tokens, k), device="cuda", generator=g)
+    elif kind == "one":  # everything at one expert
+        ids = torch.full((tokens, k), experts // 2, device="cuda")
+    elif kind == "none":
+        ids = torch.full((tokens, k), -1, device="cuda")
+    else:  # skewed, one entry in five without an expert: -1, the first id that is too large, and far off
+        ids = (torch.rand(tokens, k, device="cuda", generator=g) ** 3 * experts).long()
+        bad = torch.tensor([-1, experts, -2 ** 31, 2 ** 31 - 1], device="cuda")
+        pick = torch.randint(0, 4, (tokens, k), device="cuda", generator=g)
+        ids = torch.where(torch.rand(tokens, k, device="cuda", generator=g) < 0.2, bad[pick], ids)
+    return ids.to(dtype)
+
+
+def _order_of(ids, experts):
+    flat = ids.reshape(-1).long()
+    flat = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    at = torch.argsort(flat, stable=True)
+    row_of = torch.empty_like(at)
+    row_of[at] = torch.arange(at.numel(), device=at.device)
+    row_of[flat == experts] = -1
+    ends = torch.bincount(flat, minlength=experts + 1)[:experts].cumsum(0)
+    return torch.cat([ends.new_zeros(1), ends]).int(), row_of.reshape(ids.shape).int()
+
+
+def _check_sort(x, ids, experts, got, scale=None):
+    offsets, row_of = _order_of(ids, experts)
+    assert torch.equal(got.order.offsets, offsets) and torch.equal(got.order.row_of, row_of)
+    for source, rows in ((x, got.rows), (scale, got.scale)):
+        if source is None:
+            assert rows is None
+            continue
+        assert rows.dtype == source.dtype and rows.shape == (ids.numel(), source.shape[1])
+        raw = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[source.element_size()]
+        want = torch.zeros(rows.shape, dtype=raw, device="cuda")
+        t = torch.arange(ids.shape[0], device="cuda")[:, None].expand_as(ids)
+        has = row_of >= 0
+        want[row_of[has].long()] = source.contiguous().view(raw)[t[has]]
+        assert torch.equal(rows.view(raw), want)
+
+
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "one", "none"])
+@pytest.mark.parametrize("tokens,k,experts,hidden,dtype", [
+    (1, 1, 1, 8, torch.float16), (1, 8, 256, 7168, torch.bfloat16), (11, 2, 8, 6144, torch.float16), (32, 2, 16, 250, torch.float32),
+    (101, 4, 128, 2880, torch.float16), (37, 32, 33, 71, torch.bfloat16), (300, 3, 8192, 64, torch.float32),
+    (2047, 8, 128, 512, torch.bfloat16), (16384, 1, 5, 16, torch.float16), (2049, 8, 256, 136, torch.bfloat16),
+    (5000, 7, 64, 33, torch.float16), (40000, 4, 300, 8, torch.float32), (9000, 2, 8192, 24, torch.float16)])
+def test_sort_tokens(tokens, k, experts, hidden, dtype, kind):
+    from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
+
+    x = _randn(tokens, hidden, dtype=dtype, seed=tokens)
+    for wide in (torch.int32, torch.int64):
+        ids = _ids(tokens, k, experts, 3, kind, wide)
+        _check_sort(x, ids, experts, sort_tokens(x, ids, experts))
+
+
+@pytest.mark.parametrize("tokens,k,experts,hidden", [(1, 8, 64, 7168), (101, 4, 128, 2880), (4096, 8, 64, 1111), (3, 2, 8, 130)])
+def test_sort_tokens_e4m3_rows_with_scales(tokens, k, experts, hidden):
+    from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
+
+    x = (50 * _randn(tokens, hidden, seed=2)).to(torch.float8_e4m3fn)
+    scale = _randn(tokens, -(-hidden // 128), seed=3)
+    ids = _ids(tokens, k, experts, 4, "skewed")
+    _check_sort(x, ids, experts, sort_tokens(x, ids, experts, scale=scale), scale)
+    _check_sort(x, ids, experts, sort_tokens(x, ids, experts))
+    wide = _randn(scale.shape[1], tokens, seed=5).t()  # scales column by column
+    _check_sort(x, ids, experts, sort_tokens(x, ids, experts, scale=wide), wide)
+
+
+def test_sort_tokens_strides_alignment_and_wide_ids():
+    from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
+
+    big = _randn(50, 700, dtype=torch.bfloat16, seed=1)
+    ids = _ids(50, 4, 16, 2)
+    for lo, n in ((0, 512), (8, 512), (1, 512), (2, 130), (3, 65)):
+        x = big[:, lo:lo + n]
+        _check_sort(x, ids, 16, sort_tokens(x, ids, 16))
+    x = big[:1, :512].expand(50, 512)
+    _check_sort(x, ids, 16, sort_tokens(x, ids, 16))
+    x = _randn(512, 50, dtype=torch.bfloat16, seed=1).t()
+    _check_sort(x, ids, 16, sort_tokens(x, ids, 16))
+    columns = _ids(4, 50, 16, 2).t()  # ids that are not contiguous
+    _check_sort(big, columns, 16, sort_tokens(big, columns, 16))
+    far = ids.long() + (torch.arange(50, device="cuda")[:, None] % 2) * 2 ** 32  # in range once the upper half is lost
+    _check_sort(big, far, 16, sort_tokens(big, far, 16))
+    none = sort_tokens(big[:0], ids[:0], 16)
+    assert none.rows.shape == (0, 700) and none.order.offsets.tolist() == [0] * 17 and none.order.row_of.shape == (0, 4)
+
+
+def _unsort64(rows, row_of, weights):
+    has = row_of >= 0
+    got = rows.double()[row_of.clamp(min=0).long()] * has[:, :, None]
+    got = torch.where(has[:, :, None], got, torch.zeros((), dtype=torch.float64, device="cuda"))
+    w = weights.double()[:, :, None] if weights is not None else 1.0
+    w = torch.where(has[:, :, None], w, torch.zeros((), dtype=torch.float64, device="cuda"))
+    return got, w
+
+
+def _check_unsort(rows, row_of, weights, out):
+    got, w = _unsort64(rows, row_of, weights)
+    want, size = (got * w).sum(1), (got * w).abs().sum(1)
+    assert out.dtype == rows.dtype
+    _close(out, want, _u(rows.dtype) * want.abs() + (row_of.shape[1] + 2) * U32 * size * 2 + 2.0 ** -25, "out")
+
+
+def _check_backward(grad, rows, row_of, weights, got):
+    d_rows, d_weights = got
+    y, w = _unsort64(rows, row_of, weights)
+    has = row_of >= 0
+    g = grad.double()[:, None, :]
+    want = torch.zeros(rows.shape, dtype=torch.float64, device="cuda")
+    want[row_of[has].long()] = (g * w).expand(-1, row_of.shape[1], -1)[has]
+    if d_rows is not None:
+        assert d_rows.dtype == rows.dtype
+        _close(d_rows, want, (_u(rows.dtype) + U32) * want.abs() + 2.0 ** -25, "rows")
+    if weights is None:
+        assert d_weights is None
+    elif d_weights is not None:
+        dot, size = (g * y).sum(2), (g * y).abs().sum(2)
+        # a lane's chain of hidden / 32 terms at most, then the lanes and warps
+        _close(d_weights, dot, (rows.shape[1] / 32 + 24) * U32 * size, "weights")
+
+
+UNSORT = [(1, 1, 1, 8), (1, 8, 256, 7168), (11, 2, 8, 6144), (128, 8, 256, 512), (32, 2, 16, 250), (37, 32, 33, 71), (101, 5, 128, 2880),
+          (2047, 4, 16, 136), (300, 3, 64, 1), (9, 6, 4, 8200)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,k,experts,hidden", UNSORT)
+def test_unsort_tokens_and_gradients(tokens, k, experts, hidden, dtype):
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    for kind in ("uniform", "skewed", "none"):
+        offsets, row_of = _order_of(_ids(tokens, k, experts, 5, kind), experts)
+        order = moe_sort.ExpertOrder(offsets, row_of)
+        rows = _randn(tokens * k, hidden, dtype=dtype, seed=6)
+        weights = torch.rand(tokens, k, device="cuda", generator=_gen(7))
+        _check_unsort(rows, row_of, weights, moe_sort.unsort_tokens(rows, order, weights))
+        _check_unsort(rows, row_of, None, moe_sort.unsort_tokens(rows, order))
+        grad = _randn(tokens, hidden, dtype=dtype, seed=8)
+        _check_backward(grad, rows, row_of, weights, moe_sort.unsort_tokens_backward(grad, rows, order, weights))
+        _check_backward(grad, rows, row_of, None, moe_sort.unsort_tokens_backward(grad, rows, order))
+        _check_unsort(rows, row_of, None, moe_sort.sort_tokens_backward(rows, order))
+
+
+def test_unsort_tokens_ignores_what_has_no_row():
+    """NaN and infinities in weights without a row and in rows behind the last expert's reach nothing; where they count they show."""
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    ids = _ids(200, 4, 16, 9, "skewed")
+    offsets, row_of = _order_of(ids, 16)
+    order = moe_sort.ExpertOrder(offsets, row_of)
+    end = int(offsets[-1])
+    assert end < ids.numel()
+    for hidden in (264, 33):
+        rows = _randn(ids.numel(), hidden, dtype=torch.bfloat16, seed=1)
+        weights = torch.rand(200, 4, device="cuda", generator=_gen(2))
+        grad = _randn(200, hidden, dtype=torch.bfloat16, seed=3)
+        want = moe_sort.unsort_tokens(rows, order, weights)
+        want_rows, want_weights = moe_sort.unsort_tokens_backward(grad, rows, order, weights)
+        rows[end:] = float("nan")
+        weights[row_of < 0] = float("inf")
+        assert torch.equal(moe_sort.unsort_tokens(rows, order, weights), want)
+        d_rows, d_weights = moe_sort.unsort_tokens_backward(grad, rows, order, weights)
+        assert torch.equal(d_rows, want_rows) and torch.equal(d_weights, want_weights)
+        assert bool((d_rows[end:] == 0).all()) and bool((d_weights[row_of < 0] == 0).all())
+        empty = (row_of < 0).all(1)
+        assert bool((want[empty] == 0).all())
+        rows[0] = float("nan")
+        t = (row_of == 0).any(1)
+        out = moe_sort.unsort_tokens(rows, order, weights)
+        assert bool(out[t].isnan().all()) and not bool(out[~t].isnan().any())
+    # places that are no rows at all are skipped, whatever they say
+    wild = row_of.clone()
+    wild[0, 0], wild[1, 1], wild[2, 2] = 2 ** 31 - 1, -2 ** 31, ids.numel()
+    rows = _randn(ids.numel(), 64, dtype=torch.float32, seed=1)
+    tame = torch.where((wild < 0) | (wild >= ids.numel()), -1, wild)
+    assert torch.equal(moe_sort.unsort_tokens(rows, moe_sort.ExpertOrder(offsets, wild)),
+                       moe_sort.unsort_tokens(rows, moe_sort.ExpertOrder(offsets, tame)))
+
+
+def test_unsort_tokens_strides_alignment_and_empty():
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    offsets, row_of = _order_of(_ids(30, 4, 8, 1), 8)
+    order = moe_sort.ExpertOrder(offsets, row_of)
+    big, grads = _randn(120, 800, dtype=torch.float16, seed=1), _randn(30, 900, dtype=torch.float16, seed=2)
+    weights = torch.rand(4, 30, device="cuda", generator=_gen(2)).t()  # not contiguous
+    for lo, n in ((0, 512), (8, 512), (3, 512), (0, 77)):
+        rows, grad = big[:, lo:lo + n], grads[:, lo:lo + n]
+        _check_unsort(rows, row_of, weights, moe_sort.unsort_tokens(rows, order, weights))
+        _check_backward(grad, rows, row_of, weights, moe_sort.unsort_tokens_backward(grad, rows, order, weights))
+    one = grads[:1, :512].expand(30, 512)
+    _check_backward(one, big[:, :512], row_of, weights, moe_sort.unsort_tokens_backward(one, big[:, :512], order, weights))
+    same = torch.ones((), device="cuda", dtype=torch.float16).expand(30, 512)
+    _check_backward(same, big[:, :512], row_of, weights, moe_sort.unsort_tokens_backward(same, big[:, :512], order, weights))
+    none = moe_sort.ExpertOrder(torch.zeros(9, dtype=torch.int32, device="cuda"), row_of[:0])
+    assert moe_sort.unsort_tokens(big[:0], none, weights[:0]).shape == (0, 800)
+    d_rows, d_weights = moe_sort.unsort_tokens_backward(grads[:0, :800], big[:0], none, weights[:0])
+    assert d_rows.shape == (0, 800) and d_weights.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sort_and_unsort_through_autograd(dtype):
+    """Leaves through sort, an expert's scale, unsort: gradients of the formula, in 64 bits by autograd itself."""
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    tokens, k, experts, hidden = 60, 3, 8, 72
+    ids = _ids(tokens, k, experts, 3, "skewed", torch.int64)
+    x = _randn(tokens, hidden, dtype=dtype, seed=1).requires_grad_()
+    weights = torch.rand(tokens, k, device="cuda", generator=_gen(2)).to(dtype).requires_grad_()
+    grad = _randn(tokens, hidden, dtype=dtype, seed=4)
+    got = moe_sort.sort_tokens(x, ids, experts)
+    assert not got.order.offsets.requires_grad and not got.order.row_of.requires_grad
+    out = moe_sort.unsort_tokens(got.rows, got.order, weights)
+    out.backward(grad)
+    xd, wd = x.detach().double().requires_grad_(), weights.detach().double().requires_grad_()
+    has = (ids >= 0) & (ids < experts)
+    want = (xd[:, None, :] * (wd * has)[:, :, None]).sum(1)
+    want.backward(grad.double())
+    u = _u(dtype)
+    size = (wd * has).abs().sum(1, keepdim=True)
+    _close(out, want, ((u + 8 * U32) * size * xd.abs()).detach() + 2.0 ** -25)
+    # k rows of w * grad, rounded each, added and rounded again
+    _close(x.grad, xd.grad, ((2 * u + 8 * U32) * size * grad.double().abs()).detach() + 4 * 2.0 ** -25)
+    dot = (xd.detach().abs() * grad.double().abs()).sum(1, keepdim=True)
+    _close(weights.grad, wd.grad, u * wd.grad.abs() + (hidden / 32 + 24) * U32 * dot + 2.0 ** -25)
+    # against differences, in fp32: the output is linear in x and in the weights
+    if dtype == torch.float32:
+        for leaf in (x, weights):
+            step = _randn(*leaf.shape, seed=9)
+            moved = {id(leaf): leaf.detach() + step}
+            xs, ws = moved.get(id(x), x.detach()), moved.get(id(weights), weights.detach())
+            rows = moe_sort.sort_tokens(xs, ids, experts)
+            far = moe_sort.unsort_tokens(rows.rows, rows.order, ws)
+            change = ((far.double() - out.detach().double()) * grad.double()).sum().item()
+            assert abs(change - (leaf.grad.double() * step.double()).sum().item()) < 1e-4 * grad.numel() ** 0.5
+
+
+def test_sort_autograd_broadcast_gradients_and_unused_outputs():
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    ids = _ids(20, 2, 4, 3)
+    x = _randn(20, 48, seed=1).requires_grad_()
+    got = moe_sort.sort_tokens(x, ids, 4)
+    got.rows.sum().backward()  # an expanded gradient
+    assert torch.equal(x.grad, torch.full_like(x, 2.0))
+    base = _randn(1, 48, seed=1).requires_grad_()
+    moe_sort.sort_tokens(base.expand(20, 48), ids, 4).rows.sum().backward()  # a broadcast input: its rows' gradients add up
+    assert torch.equal(base.grad, torch.full_like(base, 40.0))
+    weights = torch.ones(20, 2, device="cuda", requires_grad=True)
+    order = got.order
+    rows = _randn(40, 48, seed=2)
+    moe_sort.unsort_tokens(rows, order, weights).sum().backward()  # only the weights want one
+    _close(weights.grad, rows.double()[order.row_of.long()].sum(2), 48 * U32 * rows.abs().max().item() * 48)
+    with torch.no_grad():
+        assert not moe_sort.sort_tokens(x, ids, 4).rows.requires_grad
+
+
+def test_sort_and_unsort_captured_and_replayed():
+    """A training step in a graph: new inputs, the same buffers; twice in one graph, each with results of its own."""
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    for tokens in (64, 5000):  # one launch, and two
+        x = _randn(tokens, 128, seed=1).requires_grad_()
+        weights = torch.rand(tokens, 4, device="cuda").requires_grad_()
+        ids = _ids(tokens, 4, 16, 2, "skewed")
+        grad = _randn(tokens, 128, seed=3)
+
+        def step():
+            got = moe_sort.sort_tokens(x, ids, 16)
+            out = moe_sort.unsort_tokens(got.rows * 2, got.order, weights)
+            return (out.detach(), *torch.autograd.grad(out, (x, weights), grad))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            first, second = step(), step()
+        for seed in (5, 6):
+            with torch.no_grad():
+                x.copy_(_randn(tokens, 128, seed=seed))
+                ids.copy_(_ids(tokens, 4, 16, seed, "skewed"))
+            graph.replay()
+            want = step()
+            for a, b, c in zip(want, first, second):
+                assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    ids = _ids(16, 2, 4, 2)
+    x = _randn(16, 64, seed=1).requires_grad_()
+    alive = (x * 2).sum()  # its graph holds x's accumulation node, of the eager stream
+    refused = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for leaf in (x, x * 1):
+            try:
+                moe_sort.sort_tokens(leaf, ids, 4)
+            except RuntimeError as e:
+                refused.append(str(e))
+    assert len(refused) == 2 and all("eager graph" in r for r in refused)
+    del alive, leaf  # (x * 1 holds the node too)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(moe_sort.sort_tokens(x, ids, 4).rows.sum(), x)
+    graph.replay()
+    assert torch.equal(got[0], torch.full_like(x, 2.0))
+
+
+def test_expert_operators_on_streams_of_their_own():
+    """Two streams at once, again and again: nothing is shared between calls."""
+    from amd_distributed_2025_b200.ops import fp8_rows, moe_sort
+
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    cases = []
+    for s, (tokens, seed) in enumerate(((6000, 1), (700, 2))):
+        x = _randn(tokens, 512, dtype=torch.bfloat16, seed=seed)
+        ids = _ids(tokens, 4, 32, seed)
+        cases.append((x, ids, moe_sort.sort_tokens(x, ids, 32), fp8_rows.rms_norm_fp8(x, x[0], residual=x)))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream, (x, ids, _, _) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append((moe_sort.sort_tokens(x, ids, 32), fp8_rows.rms_norm_fp8(x, x[0], residual=x)))
+    torch.cuda.synchronize()
+    for i, (rows, normed) in enumerate(got):
+        want_rows, want_normed = cases[i % 2][2:]
+        assert torch.equal(rows.rows, want_rows.rows) and torch.equal(rows.order.row_of, want_rows.order.row_of)
+        assert torch.equal(normed.q.view(torch.uint8), want_normed.q.view(torch.uint8)) and torch.equal(normed.total, want_normed.total)
