@@ -1,5 +1,5 @@
 // Python calls of the operators around a GPU's experts: rows with block scales (fp8_rows.h), tokens sorted by expert
-// (moe_sort.h).  Shapes and types are looked at before devices, so that a wrong call is refused without a GPU too.
+// (moe_sort.h), the experts' fp8 products (fp8_gemm.h).  Shapes and types are looked at before devices, so that a wrong call is refused without a GPU too.
 #include "bindings_experts.h"
 
 #include <ATen/MemoryOverlap.h>
@@ -10,6 +10,7 @@
 #include <unordered_set>
 
 #include "bindings_common.h"
+#include "fp8_gemm.h"
 #include "fp8_rows.h"
 #include "moe_sort.h"
 
@@ -338,6 +339,84 @@ PyObject* unsort_tokens_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------- the experts' products ----
+
+// Row-major, and at an address that a tensor map takes.
+at::Tensor for_copies(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15u) == 0 ? c : c.clone();
+}
+
+// (a, b, a_scale, b_scale, offsets, c or None, timeout_ns) -> c; None where an earlier call on the device has recorded a
+// failure, which the caller takes and raises (nothing is launched then).
+PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count_args(n, 7);
+    const at::Tensor& a_in = tensor_arg(v[0]);
+    const at::Tensor& b_in = tensor_arg(v[1]);
+    const at::Tensor& a_scale = tensor_arg(v[2]);
+    const at::Tensor& b_scale = tensor_arg(v[3]);
+    const at::Tensor& offsets_in = tensor_arg(v[4]);
+    optional<at::Tensor> c = optional_arg(v[5]);
+    const int64_t timeout_ns = int_arg(v[6]);
+    TORCH_CHECK(a_in.dim() == 2 && b_in.dim() == 3 && a_in.size(1) == b_in.size(2), "a [M, K] and b [E, N, K] must have equal K");
+    TORCH_CHECK(a_in.scalar_type() == at::kFloat8_e4m3fn && b_in.scalar_type() == at::kFloat8_e4m3fn, "a and b must be float8_e4m3fn");
+    const int64_t M = a_in.size(0), E = b_in.size(0), N = b_in.size(1), K = a_in.size(1);
+    const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
+    TORCH_CHECK(E >= 1 && E <= b200::kGroupedMaxExperts, "b must have 1 to ", num(b200::kGroupedMaxExperts), " experts, not ", num(E));
+    TORCH_CHECK(K >= 16 && K % 16 == 0, "K must be a multiple of 16");
+    TORCH_CHECK(N >= 1, "N must not be 0");
+    TORCH_CHECK(M <= INT32_MAX / 2 && E * N <= INT32_MAX / 2 && K <= INT32_MAX / 2, "the problem is too large");
+    TORCH_CHECK(a_scale.scalar_type() == at::kFloat && a_scale.dim() == 2 && a_scale.size(0) == M && a_scale.size(1) == kb,
+                "a_scale must be fp32 [M, ceil(K/128)]");
+    TORCH_CHECK(b_scale.scalar_type() == at::kFloat && b_scale.dim() == 3 && b_scale.size(0) == E && b_scale.size(1) == nb &&
+                    b_scale.size(2) == kb,
+                "b_scale must be fp32 [E, ceil(N/128), ceil(K/128)]");
+    TORCH_CHECK(offsets_in.scalar_type() == at::kInt && offsets_in.dim() == 1 && offsets_in.size(0) == E + 1, "offsets must be int32 [E + 1]");
+    if (c)
+      TORCH_CHECK(c->scalar_type() == at::kBFloat16 && c->dim() == 2 && c->size(0) == M && c->size(1) == N && c->is_contiguous(),
+                  "c must be bf16 [M, N], row-major");
+    TORCH_CHECK(timeout_ns > 0, "timeout_ms must be positive");
+    TORCH_CHECK(a_in.is_cuda(), "a must be a CUDA tensor");
+    check_device(b_in, a_in, "b");
+    check_device(a_scale, a_in, "a_scale");
+    check_device(b_scale, a_in, "b_scale");
+    check_device(offsets_in, a_in, "offsets");
+    if (c) {
+      check_device(*c, a_in, "c");
+      for (const at::Tensor* t : {&a_in, &b_in, &a_scale, &b_scale, &offsets_in}) at::assert_no_overlap(*c, *t);
+    }
+    c10::cuda::CUDAGuard guard(a_in.device());
+    if (fp8_status_code(a_in.get_device()) != 0) Py_RETURN_NONE;
+    const bool zero_rest = !c;
+    if (!c) c = new_cuda({M, N}, at::kBFloat16, a_in);
+    if (M == 0) return wrap(c);
+    const at::Tensor a = for_copies(a_in), b = for_copies(b_in), offsets = offsets_in.contiguous();
+    b200::Fp8GroupedArgs g = {};
+    g.a = a.const_data_ptr();
+    g.b = b.const_data_ptr();
+    g.a_scale = a_scale.const_data_ptr<float>();
+    g.b_scale = b_scale.const_data_ptr<float>();
+    g.offsets = offsets.const_data_ptr<int32_t>();
+    g.c = c->mutable_data_ptr();
+    g.M = (int)M;
+    g.N = (int)N;
+    g.K = (int)K;
+    g.experts = (int)E;
+    g.as_stride_m = a_scale.stride(0);
+    g.as_stride_k = a_scale.stride(1);
+    g.bs_stride_e = b_scale.stride(0);
+    g.bs_stride_n = b_scale.stride(1);
+    g.bs_stride_k = b_scale.stride(2);
+    g.zero_rest = zero_rest;
+    g.timeout_ns = (uint64_t)timeout_ns;
+    g.status = fp8_status(a.get_device());
+    g.sms = device_sms(a.get_device());
+    cuda_check(b200::launch_fp8_grouped_gemm(g, at::cuda::getCurrentCUDAStream()), "fp8_grouped_gemm launch");
+    return wrap(c);
+  });
+}
+
 // While the current stream is being captured: whether a leaf behind `t` has its gradient added up on another stream, as it
 // does when an eager graph of it is alive.  The captured backward pass would have to wait for that stream, which ends
 // the process from inside the autograd engine.
@@ -365,7 +444,7 @@ bool adds_up_elsewhere(const at::Tensor& t) {
 
 #define B200_CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kExpertCalls[] = {B200_CALL(rms_norm_fp8), B200_CALL(silu_mul_fp8), B200_CALL(sort_tokens), B200_CALL(unsort_tokens),
-                              B200_CALL(unsort_tokens_backward), {nullptr, nullptr, 0, nullptr}};
+                              B200_CALL(unsort_tokens_backward), B200_CALL(fp8_grouped_gemm), {nullptr, nullptr, 0, nullptr}};
 #undef B200_CALL
 
 }  // namespace
@@ -373,4 +452,6 @@ PyMethodDef kExpertCalls[] = {B200_CALL(rms_norm_fp8), B200_CALL(silu_mul_fp8), 
 void b200::bind_experts(py::module& m) {
   if (PyModule_AddFunctions(m.ptr(), kExpertCalls) != 0) throw py::error_already_set();
   m.def("adds_up_elsewhere", &adds_up_elsewhere);
+  m.def("fp8_grouped_tile", &b200::fp8_grouped_tile);
+  m.def("fp8_grouped_share", [](int tile, int experts) { return py::make_tuple(b200::fp8_grouped_smem(tile, experts), 512); });
 }

@@ -32,6 +32,28 @@ Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, int sms);
 
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& args, cudaStream_t stream);
 
+// The same product for the rows of many experts (see fp8_grouped_sm100.cu): row r of A in [offsets[e], offsets[e + 1]) is
+// multiplied by expert e's B.
+struct Fp8GroupedArgs {
+  const void* a;          // [M, K] e4m3, row-major
+  const void* b;          // [E, N, K] e4m3, row-major
+  const float* a_scale;   // [M, ceil(K / 128)]
+  const float* b_scale;   // [E, ceil(N / 128), ceil(K / 128)]
+  const int32_t* offsets; // [E + 1], device memory; what is out of order or out of [0, M] is cut off
+  void* c;                // [M, N] bf16 row-major
+  int M, N, K, experts;
+  long long as_stride_m, as_stride_k, bs_stride_e, bs_stride_n, bs_stride_k;  // element strides of the scale tensors
+  bool zero_rest;         // rows of C behind offsets[E] are zeroed, else left as they were
+  uint64_t timeout_ns;
+  StatusWord* status;
+  int sms;
+};
+constexpr int kGroupedMaxExperts = 1024;  // their tables lie in shared memory
+// Tokens of a tile as planned for a problem, and the shared memory of a CTA with such tiles (for tests).
+int fp8_grouped_tile(int M, int experts);
+int fp8_grouped_smem(int tile, int experts);
+cudaError_t launch_fp8_grouped_gemm(const Fp8GroupedArgs& args, cudaStream_t stream);
+
 // Self-test of the bounded wait: one warp waits for a barrier that nothing signals and leaves its record.
 cudaError_t launch_fp8_wait_selftest(StatusWord* status, uint64_t timeout_ns, cudaStream_t stream);
 

@@ -8,7 +8,9 @@ e4m3 operands, fp32 scales per row x 128-wide K block of ``a`` and per 128 x 128
 accepts the template's layout too, converting it with one transpose copy.  The scale
 tensors are read through their strides, so both layouts work without a copy.
 
-The product runs on the fp8 tensor-core path (csrc/fp8_gemm_sm100.cu).  The AMD template
+``fp8_grouped_gemm`` is the product for rows that are sorted by expert, each expert with a ``b`` of its own.
+
+The products run on the fp8 tensor-core path (csrc/fp8_gemm_sm100.cu, csrc/fp8_grouped_sm100.cu).  The AMD template
 uses the ``e4m3fnuz`` encoding; on NVIDIA hardware the type is ``torch.float8_e4m3fn``.
 """
 from __future__ import annotations
@@ -64,6 +66,31 @@ def fp8_gemm(
     while ext.fp8_gemm(a, b, a_scale, b_scale, c, int(timeout_ms * 1e6)):
         _raise_recorded(ext, a.device)  # (returns if another thread has raised it meanwhile: launch after all)
     return c
+
+
+def fp8_grouped_gemm(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    a_scale: torch.Tensor,
+    b_scale: torch.Tensor,
+    offsets: torch.Tensor,
+    c: Optional[torch.Tensor] = None,
+    timeout_ms: float = 2000.0,
+) -> torch.Tensor:
+    """The same product for the experts of one GPU: rows ``offsets[e] .. offsets[e + 1]`` of ``a [M, K]`` times ``b[e]``.
+
+    ``a`` and ``b [E, N, K]`` are ``float8_e4m3fn`` (K a multiple of 16, E <= 1024), ``a_scale [M, ceil(K/128)]`` and
+    ``b_scale [E, ceil(N/128), ceil(K/128)]`` fp32 with any strides, ``offsets [E + 1]`` int32 on the device, not
+    decreasing (``sort_tokens(...).order.offsets``); experts may have no rows.  Returns bf16 ``[M, N]``.  Rows that no
+    expert has behind ``offsets[E]`` are zero, or, in a ``c`` that is given, left as they were.
+
+    Expired waits are reported as those of ``fp8_gemm`` are: by ``check()`` or the next call on the device."""
+    ext = _ext.load()
+    while True:
+        out = ext.fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c, int(timeout_ms * 1e6))
+        if out is not None:
+            return out
+        _raise_recorded(ext, a.device)
 
 
 def _raise_recorded(ext, device: torch.device) -> None:

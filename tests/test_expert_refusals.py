@@ -96,3 +96,30 @@ def test_unsort_tokens_refusals():
     _refused("weights must be", lambda: b(grad, rows, order, F(4, 3)))
     _refused("CUDA", lambda: b(grad, rows, order, w))
     _refused("a row for each", lambda: moe_sort.sort_tokens_backward(F(7, 64), order))
+
+
+def test_fp8_grouped_gemm_refusals():
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm as f
+
+    fp8 = torch.float8_e4m3fn
+    a, b = F(4, 256).to(fp8), F(3, 130, 256).to(fp8)
+    sa, sb, off = F(4, 2), F(3, 2, 2), F(4, dtype=torch.int32)
+    _refused("equal K", lambda: f(a, b[0], sa, sb, off))
+    _refused("equal K", lambda: f(a[:, :128], b, sa, sb, off))
+    _refused("float8_e4m3fn", lambda: f(F(4, 256), b, sa, sb, off))
+    _refused("float8_e4m3fn", lambda: f(a, b.to(torch.float8_e5m2), sa, sb, off))
+    _refused("1 to 1024 experts", lambda: f(a, b[:0], sa, sb[:0], off[:1]))
+    _refused("1 to 1024 experts", lambda: f(a, F(1025, 1, 256).to(fp8), sa, F(1025, 1, 2), F(1026, dtype=torch.int32)))
+    _refused("multiple of 16", lambda: f(a[:, :24], b[:, :, :24], sa[:, :1], sb[:, :, :1], off))
+    _refused("multiple of 16", lambda: f(a[:, :0], b[:, :, :0], sa[:, :0], sb[:, :, :0], off))
+    _refused("N must not", lambda: f(a, b[:, :0], sa, sb[:, :0], off))
+    _refused("a_scale must", lambda: f(a, b, F(4, 3), sb, off))
+    _refused("a_scale must", lambda: f(a, b, sa.double(), sb, off))
+    _refused("b_scale must", lambda: f(a, b, sa, F(3, 1, 2), off))
+    _refused("b_scale must", lambda: f(a, b, sa, F(2, 2), off))
+    _refused("offsets must", lambda: f(a, b, sa, sb, off[:3]))
+    _refused("offsets must", lambda: f(a, b, sa, sb, off.long()))
+    _refused("c must", lambda: f(a, b, sa, sb, off, F(4, 130)))
+    _refused("c must", lambda: f(a, b, sa, sb, off, F(130, 4, dtype=torch.bfloat16).t()))
+    _refused("timeout_ms", lambda: f(a, b, sa, sb, off, timeout_ms=0))
+    _refused("CUDA", lambda: f(a, b, sa, sb, off))

@@ -552,3 +552,189 @@ def test_expert_operators_on_streams_of_their_own():
         want_rows, want_normed = cases[i % 2][2:]
         assert torch.equal(rows.rows, want_rows.rows) and torch.equal(rows.order.row_of, want_rows.order.row_of)
         assert torch.equal(normed.q.view(torch.uint8), want_normed.q.view(torch.uint8)) and torch.equal(normed.total, want_normed.total)
+
+
+# --------------------------------------------------------------------------------------
+# the experts' products
+# --------------------------------------------------------------------------------------
+
+def _grouped_inputs(counts, n, k, seed=1):
+    rows, experts, kb = sum(counts), len(counts), -(-k // 128)
+    g = _gen(seed)
+    a = (60 * torch.randn(max(rows, 1), k, device="cuda", generator=g)).to(torch.float8_e4m3fn)[:rows]
+    b = (60 * torch.randn(experts, n, k, device="cuda", generator=g)).to(torch.float8_e4m3fn)
+    a_scale = 0.01 + 0.02 * torch.rand(rows, kb, device="cuda", generator=g)
+    b_scale = 0.01 + 0.02 * torch.rand(experts, -(-n // 128), kb, device="cuda", generator=g)
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    return a, b, a_scale, b_scale, offsets
+
+
+def _grouped64(a, b, a_scale, b_scale, offsets):
+    """The product in 64 bits, and the sum of its terms' sizes."""
+    k, n = a.shape[1], b.shape[1]
+    ad = a.double() * a_scale.double().repeat_interleave(128, 1)[:, :k]
+    want = torch.zeros(a.shape[0], n, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(want)
+    ends = offsets.tolist()
+    for e, (lo, hi) in enumerate(zip(ends, ends[1:])):
+        bd = b[e].double() * b_scale[e].double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+        want[lo:hi] = ad[lo:hi] @ bd.T
+        size[lo:hi] = ad[lo:hi].abs() @ bd.abs().T
+    return want, size
+
+
+def _check_grouped(inputs, out):
+    want, size = _grouped64(*inputs)
+    assert out.dtype == torch.bfloat16 and out.shape == want.shape
+    # Products of a block of 128 are added up in the tensor cores in fp32 or a little less (23 bits at least are kept
+    # of the largest term: 2^-22 of the sum of sizes for 128 of them is more than it takes), then two fp32 roundings a block.
+    kb = inputs[2].shape[1]
+    _close(out, want, _u(torch.bfloat16) * want.abs() + (128 * 2.0 ** -22 + (2 * kb + 2) * U32) * size)
+
+
+GROUPED = [
+    ([1], 128, 128), ([1], 1, 16), ([0, 1], 256, 256), ([3, 0, 0, 5, 1], 130, 272), ([32] * 8, 384, 512), ([33, 31, 64, 65, 0, 1], 257, 1024),
+    ([4] * 256, 256, 640), ([0] * 100 + [7] + [0] * 155, 512, 2880), ([256], 512, 512), ([257, 255, 300, 129, 1], 264, 400),
+    ([1000, 0, 500, 3], 1000, 896), ([70] * 9, 200, 1152), ([97, 200, 10, 0, 96], 640, 384), ([1] * 1024, 64, 128),
+    ([5000, 20, 1], 300, 256), ([511, 513], 2048, 1536),
+]
+
+
+@pytest.mark.parametrize("counts,n,k", GROUPED, ids=[f"{len(c)}x{sum(c)}-{n}-{k}" for c, n, k in GROUPED])
+def test_fp8_grouped_gemm(counts, n, k):
+    from amd_distributed_2025_b200.ops import fp8_gemm as f
+
+    inputs = _grouped_inputs(counts, n, k)
+    out = f.fp8_grouped_gemm(*inputs)
+    f.check()
+    _check_grouped(inputs, out)
+    assert torch.equal(out, f.fp8_grouped_gemm(*inputs))
+    given = torch.full_like(out, 5.0)
+    assert f.fp8_grouped_gemm(*inputs, c=given) is given and torch.equal(given, out)
+
+
+def test_fp8_grouped_gemm_matches_fp8_gemm():
+    """One expert is fp8_gemm (the same sums in the same order, but the two scales are multiplied first in both)."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_gemm, fp8_grouped_gemm
+
+    a, b, a_scale, b_scale, offsets = inputs = _grouped_inputs([300], 384, 1024)
+    got, one = fp8_grouped_gemm(*inputs), fp8_gemm(a, b[0], a_scale, b_scale[0])
+    _check_grouped(inputs, got)
+    _check_grouped(inputs, one)
+
+
+def test_fp8_grouped_gemm_rows_of_no_expert():
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+
+    for n in (264, 129):
+        a, b, a_scale, b_scale, offsets = _grouped_inputs([40, 0, 30, 50], n, 256)
+        want = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+        fewer = offsets.clamp(max=70)  # the last expert's rows belong to nobody: whatever lies there is not looked at
+        a.view(torch.uint8)[70:] = 0x7F  # NaN
+        a_scale[70:] = float("nan")
+        out = fp8_grouped_gemm(a, b, a_scale, b_scale, fewer)
+        assert torch.equal(out[:70], want[:70]) and bool((out[70:] == 0).all())
+        given = torch.full_like(out, 7.0)
+        fp8_grouped_gemm(a, b, a_scale, b_scale, fewer, c=given)
+        assert torch.equal(given[:70], want[:70]) and bool((given[70:] == 7).all())
+        none = torch.zeros_like(offsets)
+        assert bool((fp8_grouped_gemm(a, b, a_scale, b_scale, none) == 0).all())
+        # offsets that are no order at all stay inside the matrices
+        fp8_grouped_gemm(a, b, a_scale, b_scale, torch.tensor([-5, 2 ** 31 - 1, -2 ** 31, 90, 400], dtype=torch.int32, device="cuda"))
+    empty = _grouped_inputs([0, 0], 64, 128)
+    assert fp8_grouped_gemm(*empty).shape == (0, 64)
+
+
+def test_fp8_grouped_gemm_strides_alignment_and_nan():
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+
+    a, b, a_scale, b_scale, offsets = _grouped_inputs([100, 3, 60], 200, 512)
+    want = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+    _check_grouped((a, b, a_scale, b_scale, offsets), want)
+    columns = a_scale.t().contiguous().t()
+    turned = b_scale.permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    assert torch.equal(fp8_grouped_gemm(a, b, columns, turned, offsets), want)
+    wide = torch.zeros(163, 528, dtype=torch.uint8, device="cuda")
+    wide[:, 16:] = a.view(torch.uint8)
+    assert torch.equal(fp8_grouped_gemm(wide.view(torch.float8_e4m3fn)[:, 16:], b, a_scale, b_scale, offsets), want)
+    shifted = torch.zeros(a.numel() + 1, dtype=torch.uint8, device="cuda")
+    shifted[1:] = a.view(torch.uint8).flatten()
+    assert torch.equal(fp8_grouped_gemm(shifted[1:].view(torch.float8_e4m3fn).view(163, 512), b, a_scale, b_scale, offsets), want)
+    room = torch.zeros(163 * 200 + 1, dtype=torch.bfloat16, device="cuda")
+    assert torch.equal(fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c=room[1:].view(163, 200)), want)
+    flat = a_scale.clone()
+    flat = torch.cat([flat.new_zeros(1), flat.flatten()])[1:].view(163, 4)  # four scales of a row that are no aligned piece
+    assert torch.equal(fp8_grouped_gemm(a, b, flat, b_scale, offsets), want)
+    a.view(torch.uint8)[101, 5] = 0x7F  # NaN stays in its row ...
+    a_scale[7, 2] = float("inf")
+    b.view(torch.uint8)[2, 9, 4] = 0x7F  # ... and in its column of its expert
+    out = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+    touched = torch.zeros_like(out, dtype=torch.bool)
+    touched[101], touched[7], touched[103:, 9] = True, True, True
+    assert bool(out[101].isnan().all()) and bool(out[103:, 9].isnan().all()) and not bool(out[7].isfinite().any())
+    assert torch.equal(out[~touched], want[~touched])
+    with pytest.raises(RuntimeError, match="overlap|memory location"):
+        both = torch.zeros(163 * 512, dtype=torch.uint8, device="cuda")
+        fp8_grouped_gemm(both.view(torch.float8_e4m3fn).view(163, 512), b, a_scale, b_scale, offsets,
+                         c=both[:163 * 400].view(torch.bfloat16).view(163, 200))
+
+
+def test_fp8_grouped_gemm_expired_wait_leaves_a_record():
+    from amd_distributed_2025_b200.ops import _ext, fp8_gemm as f
+    from amd_distributed_2025_b200.utils.status import StatusError
+
+    inputs = _grouped_inputs([5, 6], 128, 256)
+    want = f.fp8_grouped_gemm(*inputs)
+    _ext.load().fp8_wait_selftest(0, 1_000_000)  # a barrier nobody arrives on, 1 ms
+    torch.cuda.synchronize()
+    with pytest.raises(StatusError):
+        f.fp8_grouped_gemm(*inputs)
+    assert torch.equal(f.fp8_grouped_gemm(*inputs), want)
+
+
+def test_experts_of_a_layer_together():
+    """norm -> sort -> gate and up -> activation -> down -> unsort, as a layer calls them, eager and in a graph, against
+    fp32 with the same quantised rows."""
+    from amd_distributed_2025_b200.ops import fp8_rows, moe_sort
+    from amd_distributed_2025_b200.ops.fp8_gemm import check, fp8_grouped_gemm
+
+    tokens, k, experts, hidden, inner = 150, 4, 16, 512, 384
+    g = _gen(3)
+    x = torch.randn(tokens, hidden, device="cuda", generator=g).bfloat16()
+    residual = torch.randn(tokens, hidden, device="cuda", generator=g).bfloat16()
+    weight = torch.ones(hidden, device="cuda", dtype=torch.bfloat16)
+    _, up, _, up_scale, _ = _grouped_inputs([1] * experts, 2 * inner, hidden, 5)
+    _, down, _, down_scale, _ = _grouped_inputs([1] * experts, hidden, inner, 6)
+    up_scale, down_scale = up_scale * 0.02, down_scale * 0.02
+    ids = _ids(tokens, k, experts, 4, "skewed")
+    routing = torch.rand(tokens, k, device="cuda", generator=g)
+
+    def layer():
+        normed = fp8_rows.rms_norm_fp8(x, weight, residual=residual)
+        rows = moe_sort.sort_tokens(normed.q, ids, experts, scale=normed.scale)
+        inside = fp8_grouped_gemm(rows.rows, up, rows.scale, up_scale, rows.order.offsets)
+        q, scale = fp8_rows.silu_mul_fp8(inside)
+        y = fp8_grouped_gemm(q, down, scale, down_scale, rows.order.offsets)
+        return normed, rows, inside, q, scale, y, moe_sort.unsort_tokens(y, rows.order, routing)
+
+    normed, rows, inside, q, scale, y, out = layer()
+    check()
+    end = int(rows.order.offsets[-1])
+    assert 0 < end < tokens * k
+    # each step on the one before it
+    _check_norm(x, weight, residual, normed)
+    _check_sort(normed.q, ids, experts, rows_of := moe_sort.SortedTokens(rows.rows, rows.scale, rows.order), normed.scale)
+    _check_grouped((rows_of.rows, up, rows.scale, up_scale, rows.order.offsets), inside)
+    _check_silu(inside, (q, scale))
+    _check_grouped((q, down, scale, down_scale, rows.order.offsets), y)
+    _check_unsort(y, rows.order.row_of, routing, out)
+    assert bool((out[(rows.order.row_of < 0).all(1)] == 0).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = layer()[-1]
+    for seed in (7, 8):
+        x.copy_(_randn(tokens, hidden, dtype=torch.bfloat16, seed=seed))
+        ids.copy_(_ids(tokens, k, experts, seed, "skewed"))
+        graph.replay()
+        assert torch.equal(captured, layer()[-1])
+    check()
