@@ -2,25 +2,42 @@
 //   C[r, n] = sum_kb (A_kb[r, :] . B_e,kb[n, :]) * as[r, kb] * bs[e, n / 128, kb]   for r in [offsets[e], offsets[e + 1])
 // Rows of A are sorted by expert and packed; the offsets are device memory, so nothing waits for the host.
 //
-// An expert has a few rows or a few hundred, and never a whole number of tiles.  The weights take the side of the tensor
-// cores' instruction whose size is fixed (a CTA pair has 256 rows of an expert's B, cta_group::2), the tokens the side
-// whose size is free: a tile is cut to the rows that its expert has left, in steps of 32.  So the accumulators lie with
-// output columns in tensor-memory lanes and tokens in columns.  In that order a token's scale belongs to a column, and read with a
-// lane to a row every lane would need the scale of every column.  The epilogue reads 16 lanes x 256 bits instead, which
-// gives a thread the same two columns of every eight for each of its four rows: one 16-byte read of scales (already
-// multiplied by the weights' scale, and laid out in that order, by the two warps that bring them in) serves sixteen sums.
-// The same layout is what stmatrix transposes on the way out, to rows of C.
+// A CTA pair (cta_group::2) multiplies 256 output columns of an expert by some of its rows.  Which of the two is which side
+// of the tensor cores' instruction goes by how many rows there are (two kernels, chosen by the mean):
+//   WIDE    Tokens are the rows of the product, 256 of them, or 128 where an expert has no more left.  A token lies in a
+//           tensor-memory lane, so its scale is one number to an epilogue thread and K block.
+//   else    Output columns are the rows, tokens the side whose size is free: 32 or 64.  What counts is that the weights
+//           stream: eight stages of 16 KB of them lie ahead in each SM.  A token's scale belongs to a column then; the
+//           epilogue reads 16 lanes x 128 bits of tensor memory at a time, which gives a thread every fourth token, and so eight
+//           scales for sixteen sums instead of a scale a sum.  stmatrix turns the result around on its way out.
+// Scales come in by two warps, which multiply both operands' and lay them out as the epilogue reads them.
 //
-// Every 128-wide K block is multiplied into a tensor-memory buffer of its own; eight epilogue warps (two per lane quarter,
-// which take 32-token chunks in turn) multiply by the scales and accumulate in fp32 registers while the next buffer is
-// being filled.  Pairs are persistent, and walk the same list of tiles: experts in order, an expert's weight tiles in
-// order, its token tiles innermost, so that pairs at work at the same time share weights in L2.
+// Every 128-wide K block is multiplied into tensor memory of its own: two buffers of 256 columns, each for one K block (256
+// tokens), two (128) or four.  Eight epilogue warps, two to a lane quarter, take a buffer out, hand it back, and add it up in
+// fp32 registers while the other is being filled.  Pairs are persistent, and walk the same list of tiles: experts in order,
+// an expert's weight tiles in order, its token tiles innermost, so that pairs at work at the same time share weights in L2.
+//
+// What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 537 us, 7.0
+// TB/s in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x 4096, one expert: 123 us
+// both, 2.2 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights) is between the two, 480 us.
+// What it took, us at 8192 rows of one expert / of 64 experts / at 256 experts with 4 rows each:
+//   tokens always on the free side, up to 256 of them, 16 x 256 bits           154 / 232 / 570
+//   the next piece out of tensor memory while one is added up                  176 / 208 / 552   (registers spill)
+//   256 tokens as rows                                                         128 / 224 / 537
+//   16 x 128 bits instead (the tensor memory gives those four times as fast)   127 / 221 / 537
+//   buffers emptied at once and handed back before the sums                    120 / 220 / 537
+//   128 tokens as rows                                                         123 / 200 / 537
+// Shared memory is what the free side runs short of: sixteen-byte reads take four passes each beside what the tensor cores
+// read (920 cycles for the sums of a buffer that take 240 without them; asked for a half ahead, 650).  A spilled register in
+// the loop costs more the more shared memory is taken, as L1 is what is left of it.  L2 prefetches of weights ahead of the
+// copies: 530 to 590 and more in the last column.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_gemm.h"
 #include "fp8_pipeline.cuh"
@@ -41,13 +58,15 @@ constexpr int kChunk = 32;  // tokens of a chunk; a tile is a whole number of th
 constexpr int kEpiWarps = 8;
 constexpr int kScaleWarps = 2;
 constexpr int kThreads = 64 + 32 * (kScaleWarps + kEpiWarps);
-constexpr int kLightRegs = 56, kEpiRegs = 224;
+constexpr int kLightRegs = 40, kEpiRegs = 232;
 static_assert(128 * kLightRegs + 256 * kEpiRegs == kThreads * 168, "not more than the block is launched with");
-constexpr int kMaxStages = 12;
-constexpr int kMaxBufs = 4;
+// More stages do not pay: what they take is taken from L1, which the scales come through.
+constexpr int kMaxStages = 8, kWideStages = 5;
+constexpr int kBufs = 2;        // tensor-memory buffers of 256 columns
+constexpr uint32_t kBufCols = 256;
 constexpr int kGroup = 4;       // K blocks whose scales come in together
-constexpr int kScaleSlots = 3;
-constexpr int kSlabBytes = 16 * 64;  // per epilogue warp: 16 tokens x 32 output columns
+constexpr int kScaleSlots = 4;
+constexpr int kSlabBytes = 2048;  // per epilogue warp: 32 tokens x 32 output columns
 constexpr int kBarBytes = 512;
 constexpr int kMaxDynamicSmem = 232448 - 256;
 constexpr int kTmemCols = 512;
@@ -72,7 +91,7 @@ struct GroupedParams {
 struct Tile {
   int expert, nt;
   int row0, rows;  // of A
-  int width;       // rows, rounded up to whole chunks
+  int width;       // tokens that are brought in and multiplied: 256, 128, or rows rounded up to whole chunks
 };
 
 // The experts' rows and the number of tiles up to and including each, in shared memory.
@@ -90,33 +109,28 @@ struct Walk {
     const int local = tile - (e > 0 ? t.tiles_end[e - 1] : 0);
     const int count = t.count[e];
     const int parts = (count + BT - 1) / BT;
-    const int each = ((count + parts - 1) / parts + kChunk - 1) / kChunk * kChunk;  // tiles of an expert are of one size
     Tile r;
     r.expert = e;
     r.nt = local / parts;
     const int part = local - r.nt * parts;
-    r.row0 = t.start[e] + part * each;
-    r.rows = min(each, count - part * each);
-    r.width = (r.rows + kChunk - 1) / kChunk * kChunk;
+    r.row0 = t.start[e] + part * BT;
+    r.rows = min(BT, count - part * BT);
+    r.width = BT == 64 ? (r.rows + kChunk - 1) / kChunk * kChunk : r.rows > kRows ? 2 * kRows : kRows;
     return r;
   }
 };
 
-// Where a token's scale lies among those of its 16: a lane's four (columns 2 q, 2 q + 1 of both groups of eight) side by side.
-__device__ __forceinline__ int scale_place(int token) {
-  return (token & ~15) | ((token >> 1 & 3) << 2) | ((token >> 3 & 1) << 1) | (token & 1);
-}
+// Where a token's scale lies among those of its chunk: a lane's eight (every fourth token) side by side.
+__device__ __forceinline__ int scale_place(int token) { return (token & ~31) | ((token & 3) << 3) | (token >> 2 & 7); }
 
 }  // namespace
 
-// CH: 32-token chunks of an epilogue warp; a tile has up to 64 * CH tokens.
-template <int CH>
+// WIDE: tiles of up to 256 tokens, else of up to 64.
+template <bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_big,
                    const __grid_constant__ CUtensorMap map_small, const GroupedParams p) {
-  constexpr int kBt = 64 * CH;
-  constexpr int kBufs = kBt == 256 ? 2 : kMaxBufs;
-  constexpr uint32_t kBufCols = kBt;
+  constexpr int kBt = WIDE ? 256 : 64;
   constexpr uint32_t kStageBytes = kWeightBytes + kBt / 2 * kBlockK;
   constexpr uint32_t kSlotBytes = kGroup * kBt * 4;
   extern __shared__ uint8_t smem_raw[];
@@ -141,9 +155,9 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   auto full_bar = [&](uint32_t s) { return bars + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bars + 8u * (kMaxStages + s); };
   auto tfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + s); };
-  auto tempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + kMaxBufs + s); };
-  auto sfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kMaxBufs + s); };
-  auto sempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kMaxBufs + kScaleSlots + s); };
+  auto tempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + kBufs + s); };
+  auto sfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + s); };
+  auto sempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + kScaleSlots + s); };
 
   if (tid == 0) {
     abort_flag = 0;
@@ -204,6 +218,8 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   const int total = tables.tiles_end[p.experts - 1];
   const int first_tile = (int)blockIdx.x >> 1, tile_step = (int)gridDim.x >> 1;
   Walk<kBt> walk{tables, p.n_tiles};
+  // K blocks that are multiplied into a tensor-memory buffer one beside the other.
+  auto steps = [](int width) { return WIDE ? 2 * kRows / width : 4; };
 
   // All of a CTA's threads come here in the end, each role on its own way: no CTA retires while the other may still signal
   // its barriers.
@@ -254,28 +270,34 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
         for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
           const Tile t = walk.at(tile);
-          const uint32_t idesc = make_idesc_e4m3_f32(256, t.width);
+          const uint32_t idesc = WIDE ? make_idesc_e4m3_f32(t.width, 2 * kRows) : make_idesc_e4m3_f32(2 * kRows, t.width);
+          const int step = steps(t.width);
+          const uint32_t block_cols = kBufCols / (uint32_t)step;
           bool ok = true;
-          for (int kb = 0; kb < p.k_blocks && ok; ++kb) {
-            ok = fp8_wait(tempty_bar(buf), buf_phase ^ 1u, &abort_flag, p, 200 + (int)buf) &&
-                 fp8_wait(full_bar(stage), phase, &abort_flag, p, 300 + (int)stage);
-            if (!ok) break;
+          for (int kb = 0; kb < p.k_blocks && ok; kb += step) {
+            ok = fp8_wait(tempty_bar(buf), buf_phase ^ 1u, &abort_flag, p, 200 + (int)buf);
             ptx::tcgen05_fence_after();
-            const uint32_t sa = base + stage * kStageBytes;
-            const uint64_t da = ptx::make_smem_desc_k_sw128(sa);
-            const uint64_t db = ptx::make_smem_desc_k_sw128(sa + kWeightBytes);
-            const uint32_t d = tmem_base + buf * kBufCols;
-            if (ptx::elect_one()) {
+            const int here = min(step, p.k_blocks - kb);
+            for (int i = 0; i < here; ++i) {
+              ok = ok && fp8_wait(full_bar(stage), phase, &abort_flag, p, 300 + (int)stage);
+              if (!ok) break;
+              ptx::tcgen05_fence_after();
+              const uint32_t sa = base + stage * kStageBytes;
+              const uint64_t da = ptx::make_smem_desc_k_sw128(WIDE ? sa + kWeightBytes : sa);
+              const uint64_t db = ptx::make_smem_desc_k_sw128(WIDE ? sa : sa + kWeightBytes);
+              const uint32_t d = tmem_base + buf * kBufCols + (uint32_t)i * block_cols;
+              if (ptx::elect_one()) {
 #pragma unroll
-              for (int j = 0; j < kBlockK / 32; ++j)  // 32 fp8 of K = 32 bytes = 2 descriptor address units
-                umma_fp8_pair(d, da + 2u * j, db + 2u * j, idesc, j > 0 ? 1u : 0u);
-              ptx::umma_commit_pair(empty_bar(stage), 3);
-              ptx::umma_commit_pair(tfull_bar(buf), 3);
-            }
-            __syncwarp();
-            if (++stage == (uint32_t)p.stages) {
-              stage = 0;
-              phase ^= 1u;
+                for (int j = 0; j < kBlockK / 32; ++j)  // 32 fp8 of K = 32 bytes = 2 descriptor address units
+                  umma_fp8_pair(d, da + 2u * j, db + 2u * j, idesc, j > 0 ? 1u : 0u);
+                ptx::umma_commit_pair(empty_bar(stage), 3);
+                if (i + 1 == here) ptx::umma_commit_pair(tfull_bar(buf), 3);
+              }
+              __syncwarp();
+              if (++stage == (uint32_t)p.stages) {
+                stage = 0;
+                phase ^= 1u;
+              }
             }
             if (++buf == (uint32_t)kBufs) {
               buf = 0;
@@ -286,19 +308,24 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         }
       }
     } else {
-      // ---- scales: those of four K blocks for up to CH tokens a lane, times the weights' --------------------
+      // ---- scales: those of four K blocks for up to two tokens a lane, times the weights' ---------------------
+      // WIDE: tokens of this CTA's rows, as they come, once for each block of weights; else in the order in which the
+      // epilogue's lanes read them.
       const int l = (warp - 2) * 32 + lane;
       uint32_t slot = 0, phase = 0;
       for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
         const Tile t = walk.at(tile);
-        const float* bs = p.b_scale + t.expert * p.bs_stride_e + min(t.nt * 2 + cta, (p.N - 1) >> 7) * p.bs_stride_n;
+        const int last = (p.N - 1) >> 7;
+        const float* bs = p.b_scale + t.expert * p.bs_stride_e;
+        const float* b0 = bs + min(t.nt * 2 + (WIDE ? 0 : cta), last) * p.bs_stride_n;
+        const float* b1 = bs + min(t.nt * 2 + 1, last) * p.bs_stride_n;
+        const int token0 = WIDE ? cta * (t.width / 2) : 0;
         for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
-          float b[kGroup], s[CH][kGroup];
+          float s[2][kGroup];
 #pragma unroll
-          for (int i = 0; i < kGroup; ++i) b[i] = __ldg(bs + min(kb + i, p.k_blocks - 1) * p.bs_stride_k);
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            const int token = l + 64 * c;
+          for (int c = 0; c < 2; ++c) {
+            if (c == 1 && !(WIDE && t.width == 2 * kRows)) break;
+            const int token = token0 + l + 64 * c;
             const float* as = p.a_scale + (long long)min(t.row0 + token, p.M - 1) * p.as_stride_m;
             if (token >= t.rows) {
 #pragma unroll
@@ -311,18 +338,28 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
               for (int i = 0; i < kGroup; ++i) s[c][i] = __ldg(as + min(kb + i, p.k_blocks - 1) * p.as_stride_k);
             }
           }
+          float b[2][kGroup];
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            b[0][i] = __ldg(b0 + min(kb + i, p.k_blocks - 1) * p.bs_stride_k);
+            if (WIDE) b[1][i] = __ldg(b1 + min(kb + i, p.k_blocks - 1) * p.bs_stride_k);
+          }
           if (!fp8_wait(sempty_bar(slot), phase ^ 1u, &abort_flag, p, 500 + (int)slot)) break;
           const uint32_t at = scales + slot * kSlotBytes;
+          auto put = [&](int place, const float* f, const float* w) {
 #pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            const int token = l + 64 * c;
-            if (token < t.width) {
-#pragma unroll
-              for (int i = 0; i < kGroup; ++i)
-                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(i * kBt + scale_place(token)) * 4u),
-                             "f"(s[c][i] * b[i])
-                             : "memory");
+            for (int i = 0; i < kGroup; ++i)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(i * kBt + place) * 4u), "f"(f[i] * w[i]) : "memory");
+          };
+          if (WIDE) {
+            put(l, s[0], b[0]);
+            put(kRows + l, s[0], b[1]);
+            if (t.width == 2 * kRows) {
+              put(l + 64, s[1], b[0]);
+              put(kRows + l + 64, s[1], b[1]);
             }
+          } else {
+            put(scale_place(l), s[0], b[0]);
           }
           ptx::mbar_arrive(sfull_bar(slot));
           if (++slot == kScaleSlots) {
@@ -340,118 +377,271 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   ptx::setmaxnreg_inc<kEpiRegs>();
   const int ew = warp - 2 - kScaleWarps;
   const int q = warp & 3;
-  const int side = ew >> 2;  // chunks side, side + 2, ... of a tile
+  const int side = ew >> 2;  // which half of the columns (else: which of a tile's two chunks) is this warp's
   {
     const uint32_t slab = slabs + (uint32_t)ew * kSlabBytes;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(side * kChunk);
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t leader_tempty = ptx::map_cluster(tempty_bar(0), 0);
-    const uint32_t scale_at = scales + (uint32_t)(side * kChunk + (lane & 3) * 4) * 4u;
-    uint32_t buf = 0, buf_phase = 0, slot = 0, slot_phase = 0;
+    uint32_t bufs = 0, slots = 0;  // used so far: the low bits say which one is next, the bit above them its phase
     bool alive = true;
-    for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
-      const Tile t = walk.at(tile);
-      const int n0 = t.nt * 2 * kRows + cta * kRows + q * 32;
-      const int chunks = n0 < p.N ? (t.width / kChunk - side + 1) >> 1 : 0;  // of this warp
-      float2 acc[CH][2][4][2];  // [chunk][16 lanes][8 tokens][8 lanes]: the sums of two neighbouring tokens
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[c][x >> 3][x >> 1 & 3][x & 1] = make_float2(0.f, 0.f);
+    auto arrive_done = [&]() {  // the buffer is free for the next products (the warp is converged, and its reads are complete)
+      ptx::tcgen05_fence_before();
+      ptx::mbar_arrive_remote_if(lane == 0, leader_tempty + 8u * (bufs & 1u));
+    };
+    auto await_products = [&]() {
+      alive &= fp8_wait(tfull_bar(bufs & 1u), bufs >> 1 & 1u, &abort_flag, p, 400 + (int)(bufs & 1u));
+      __syncwarp();
+      ptx::tcgen05_fence_after();
+    };
+    auto await_scales = [&]() {
+      alive &= fp8_wait(sfull_bar(slots % kScaleSlots), slots / kScaleSlots & 1u, &abort_flag, p, 600 + (int)(slots % kScaleSlots));
+      __syncwarp();
+    };
+    auto free_scales = [&]() {
+      __syncwarp();
+      ptx::mbar_arrive_if(lane == 0, sempty_bar(slots % kScaleSlots));
+      ++slots;
+    };
+    // 32 tokens x 32 columns leave through the slab, 64 bytes to a token (its four pieces swapped so that neither way meets
+    // bank conflicts), in pieces of 16 bytes, four lanes to a token.
+    auto piece_at = [&](int row, int piece) { return slab + (uint32_t)row * 64u + (uint32_t)((piece ^ (row >> 1 & 3)) << 4); };
+    auto send = [&](int row0, int rows, int n0) {
+      __syncwarp();
+      rows = min(rows, 32);
+      if (p.vec_out) {
+        const int n = n0 + (lane & 3) * 8;
+        if (n < p.N) {
+          __nv_bfloat16* to = p.c + (long long)(row0 + (lane >> 2)) * p.N + n;
+#pragma unroll 4
+          for (int row = lane >> 2; row < rows; row += 8) {
+            uint4 w;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                         : "r"(piece_at(row, lane & 3))
+                         : "memory");
+            *reinterpret_cast<uint4*>(to) = w;
+            to += 8ll * p.N;
+          }
+        }
+      } else if (n0 + lane < p.N) {  // a column to a lane
+        uint16_t* to = reinterpret_cast<uint16_t*>(p.c) + (long long)row0 * p.N + n0 + lane;
 #pragma unroll 1
-      for (int kb = 0; kb < p.k_blocks; ++kb) {
-        const int g = kb % kGroup;
-        if (g == 0) alive &= fp8_wait(sfull_bar(slot), slot_phase, &abort_flag, p, 600 + (int)slot);
-        alive &= fp8_wait(tfull_bar(buf), buf_phase, &abort_flag, p, 400 + (int)buf);
-        __syncwarp();
-        ptx::tcgen05_fence_after();
-        auto done = [&]() {  // the buffer is free for the next products (the warp is converged, and its reads are complete)
-          ptx::tcgen05_fence_before();
-          ptx::mbar_arrive_remote_if(lane == 0, leader_tempty + 8u * buf);
-        };
-        if (chunks == 0) done();
-        const uint32_t s_at = scale_at + slot * kSlotBytes + (uint32_t)(g * kBt * 4);
-#pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-          if (c < chunks) {
-            constexpr int kAtOnce = CH > 1 ? 2 : 1;
-            uint32_t v[kAtOnce][2][16];
-            float s[kAtOnce][8];
-#pragma unroll
-            for (int d = 0; d < kAtOnce; ++d) {
-              // (a chunk behind the tile's last is read and added up too: its columns lie in the buffer, its sums go nowhere)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                ptx::tmem_ld_16x256b_x4(lane_addr + ((uint32_t)(h * 16) << 16) + buf * kBufCols + (c + d) * 2 * kChunk, v[d][h]);
-              ld_shared_f4(s[d], s_at + (uint32_t)((c + d) * 2 * kChunk) * 4u);
-              ld_shared_f4(s[d] + 4, s_at + (uint32_t)((c + d) * 2 * kChunk + 16) * 4u);
-            }
-            ptx::tmem_ld_wait();
-            if (c + 2 >= chunks) done();
-#pragma unroll
-            for (int d = 0; d < kAtOnce; ++d)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 ss = make_float2(s[d][2 * i], s[d][2 * i + 1]);
-                  fma2(acc[c + d][h][i][0], v[d][h][4 * i], v[d][h][4 * i + 1], ss);
-                  fma2(acc[c + d][h][i][1], v[d][h][4 * i + 2], v[d][h][4 * i + 3], ss);
-                }
-          }
-        }
-        if (g == kGroup - 1 || kb + 1 == p.k_blocks) {
-          __syncwarp();
-          ptx::mbar_arrive_if(lane == 0, sempty_bar(slot));
-          if (++slot == kScaleSlots) {
-            slot = 0;
-            slot_phase ^= 1u;
-          }
-        }
-        if (++buf == (uint32_t)kBufs) {
-          buf = 0;
-          buf_phase ^= 1u;
+        for (int row = 0; row < rows; ++row) {
+          uint16_t w;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(piece_at(row, lane >> 3) + (uint32_t)(lane & 7) * 2u) : "memory");
+          *to = w;
+          to += p.N;
         }
       }
-      alive = __all_sync(0xffffffffu, alive);
-      if (!alive) break;
-      // ---- result: 16 tokens at a time through the slab, 64 bytes of a row to four lanes ---------------------
+      __syncwarp();
+    };
+    for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
+      const Tile t = walk.at(tile);
+      if (WIDE && t.width == 2 * kRows) {
+        // ---- tokens in lanes: a lane's scale is its token's times that of its columns' block of weights -------
+        // A CTA has 128 of 256 tokens in its lanes; `side` is the block of weights.
+        const bool idle = t.rows <= cta * kRows + q * 32 || t.nt * 2 * kRows + side * kRows >= p.N;
+        const uint32_t from = lane_addr + (uint32_t)(side * kRows);
+        const uint32_t scale_at = scales + (uint32_t)(side * kRows + q * 32 + lane) * 4u;
+        float2 acc[4][16];
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (c >= chunks) break;
-        const int token0 = (2 * c + side) * kChunk;
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i0 = 0; i0 < 4; i0 += 2) {
+          for (int x = 0; x < 16; ++x) acc[c][x] = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          const int g = kb % kGroup;
+          if (g == 0) await_scales();
+          float s;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(s)
+                       : "r"(scale_at + slots % kScaleSlots * kSlotBytes + (uint32_t)(g * kBt * 4))
+                       : "memory");
+          await_products();
+          if (!idle) {
 #pragma unroll
-          for (int i = i0; i < i0 + 2; ++i) {
-            const int row = (i - i0) * 8 + (lane & 7);  // of the slab: a token
-            const uint32_t at = slab + (uint32_t)row * 64u + (uint32_t)(((lane >> 3) ^ (row >> 1 & 3)) << 4);
-            ptx::stmatrix_x4_trans(at, pack2(acc[c][0][i][0]), pack2(acc[c][0][i][1]), pack2(acc[c][1][i][0]),
-                                   pack2(acc[c][1][i][1]));
+            for (int c = 0; c < 4; c += 2) {
+              uint32_t v[2][32];
+              ptx::tmem_ld_32x32b_x32(from + (bufs & 1u) * kBufCols + c * 32, v[0]);
+              ptx::tmem_ld_32x32b_x32(from + (bufs & 1u) * kBufCols + c * 32 + 32, v[1]);
+              ptx::tmem_ld_wait();
+              if (c == 2) arrive_done();
+#pragma unroll
+              for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) fma2(acc[c + d][x], v[d][2 * x], v[d][2 * x + 1], make_float2(s, s));
+            }
+          } else {
+            arrive_done();
           }
-          __syncwarp();
+          ++bufs;
+          if (g == kGroup - 1 || kb + 1 == p.k_blocks) free_scales();
+        }
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        if (!idle) {
+          const Tile t = walk.at(tile);  // (worked out again: what it takes to keep it through the loop is needed there)
+          const int first = cta * kRows + q * 32, rows = t.rows - first, n0 = t.nt * 2 * kRows + side * kRows;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int row = (lane >> 2) + 8 * j, piece = lane & 3;
-            uint32_t v[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                         : "r"(slab + (uint32_t)row * 64u + (uint32_t)((piece ^ (row >> 1 & 3)) << 4))
+          for (int c = 0; c < 4; ++c) {
+            if (n0 + c * 32 < p.N) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(lane, j)),
+                             "r"(pack2(acc[c][4 * j])), "r"(pack2(acc[c][4 * j + 1])), "r"(pack2(acc[c][4 * j + 2])),
+                             "r"(pack2(acc[c][4 * j + 3]))
+                             : "memory");
+              send(t.row0 + first, rows, n0 + c * 32);
+            }
+          }
+        }
+        continue;
+      }
+      if constexpr (WIDE) {
+        // ---- the same for up to 128 tokens: a CTA has 64 of them in its lanes, once with each block of weights, whose
+        // columns `side` halves; two K blocks to a buffer
+        const bool idle = t.rows <= cta * (kRows / 2) + (q & 1) * 32 || t.nt * 2 * kRows + (q >> 1) * kRows + side * 64 >= p.N;
+        const uint32_t from = lane_addr + (uint32_t)(side * 64);
+        const uint32_t scale_at = scales + (uint32_t)((q >> 1) * kRows + (q & 1) * 32 + lane) * 4u;
+        float2 acc[2][16];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[c][x] = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int kb = 0; kb < p.k_blocks; kb += 2) {
+          const int g = kb % kGroup;
+          if (g == 0) await_scales();
+          float s[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            asm volatile("ld.shared.f32 %0, [%1];"
+                         : "=f"(s[i])
+                         : "r"(scale_at + slots % kScaleSlots * kSlotBytes + (uint32_t)((g + i) * kBt * 4))
                          : "memory");
-            const int token = token0 + i0 * 8 + row, n = n0 + piece * 8;
-            if (token < t.rows && n < p.N) {
-              __nv_bfloat16* to = p.c + (long long)(t.row0 + token) * p.N + n;
-              if (p.vec_out) {
-                *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-              } else {
+          const bool both = kb + 1 < p.k_blocks;  // of the buffer's blocks; one that is not there is read as it is, and left
+          await_products();
+          if (!idle) {
+            uint32_t v[4][32];
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                  if (n + x < p.N) reinterpret_cast<uint16_t*>(to)[x] = (uint16_t)(v[x >> 1] >> (16 * (x & 1)));
+            for (int j = 0; j < 4; ++j) ptx::tmem_ld_32x32b_x32(from + (bufs & 1u) * kBufCols + (j >> 1) * 128 + (j & 1) * 32, v[j]);
+            ptx::tmem_ld_wait();
+            arrive_done();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j < 2 || both) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) fma2(acc[j & 1][x], v[j][2 * x], v[j][2 * x + 1], make_float2(s[j >> 1], s[j >> 1]));
+              }
+            }
+          } else {
+            arrive_done();
+          }
+          ++bufs;
+          if (g == kGroup - 2 || kb + 2 >= p.k_blocks) free_scales();
+        }
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        if (!idle) {
+          const Tile t = walk.at(tile);
+          const int first = cta * (kRows / 2) + (q & 1) * 32, rows = t.rows - first;
+          const int n0 = t.nt * 2 * kRows + (q >> 1) * kRows + side * 64;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (n0 + c * 32 < p.N) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(lane, j)),
+                             "r"(pack2(acc[c][4 * j])), "r"(pack2(acc[c][4 * j + 1])), "r"(pack2(acc[c][4 * j + 2])),
+                             "r"(pack2(acc[c][4 * j + 3]))
+                             : "memory");
+              send(t.row0 + first, rows, n0 + c * 32);
+            }
+          }
+        }
+        continue;
+      }
+      // ---- output columns in lanes, a chunk of tokens to a warp; four K blocks to a buffer, 64 columns apart ----
+      const int n0 = t.nt * 2 * kRows + cta * kRows + q * 32;
+      if (n0 >= p.N || side * kChunk >= t.width) {  // nothing of the tile is this warp's
+#pragma unroll 1
+        for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+          await_scales();
+          await_products();
+          arrive_done();
+          ++bufs;
+          free_scales();
+        }
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        continue;
+      }
+      const uint32_t from = lane_addr + (uint32_t)(side * kChunk);
+      const uint32_t scale_at = scales + (uint32_t)(side * kChunk + (lane & 3) * 8) * 4u;
+      float2 acc[2][8];  // [16 lanes][4 tokens]: the sums of a token for two columns, 8 apart
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[x >> 3][x & 7] = make_float2(0.f, 0.f);
+      // Two K blocks at a time.  Their scales are asked for two blocks ahead: beside the tensor cores, which read their
+      // operands from shared memory, a load from there takes longer than the sums.
+      float s[2][2][8];
+      auto fetch = [&](int kb, float (&to)[2][8]) {
+        if (kb % kGroup == 0) {
+          if (kb > 0) free_scales();
+          await_scales();
+        }
+        const uint32_t s_at = scale_at + slots % kScaleSlots * kSlotBytes + (uint32_t)(kb % kGroup * kBt * 4);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          ld_shared_f4(to[d], s_at + (uint32_t)(d * kBt * 4));
+          ld_shared_f4(to[d] + 4, s_at + (uint32_t)(d * kBt * 4) + 16u);
+        }
+      };
+      fetch(0, s[0]);
+#pragma unroll 1
+      for (int kb0 = 0; kb0 < p.k_blocks; kb0 += kGroup) {
+        await_products();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int kb = kb0 + 2 * u;
+          if (kb < p.k_blocks) {
+            uint32_t v[2][2][16];
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                ptx::tmem_ld_16x128b_x8(from + ((uint32_t)(h * 16) << 16) + (bufs & 1u) * kBufCols + (2 * u + d) * 64, v[d][h]);
+            ptx::tmem_ld_wait();
+            if (u == 1 || kb + 2 >= p.k_blocks) {
+              arrive_done();
+              ++bufs;
+            }
+            if (kb + 2 < p.k_blocks) fetch(kb + 2, s[u ^ 1]);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              if (kb + d < p.k_blocks) {  // (the place of a block that is not there is read as it is)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+                    fma2(acc[h][i], v[d][h][2 * i], v[d][h][2 * i + 1], make_float2(s[u][d][i], s[u][d][i]));
               }
             }
           }
-          __syncwarp();
         }
       }
+      free_scales();
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      const int token0 = side * kChunk;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {  // eight tokens (a lane's are four apart), 32 columns
+        const auto two = [&](int h, bool upper) {
+          return pack2(upper ? make_float2(acc[h][i].y, acc[h][i + 1].y) : make_float2(acc[h][i].x, acc[h][i + 1].x));
+        };
+        const int token = 4 * i + ((lane & 1) << 2) + (lane >> 1 & 3);
+        ptx::stmatrix_x4_trans(piece_at(token, lane >> 3), two(0, false), two(0, true), two(1, false), two(1, true));
+      }
+      send(t.row0 + token0, t.rows - token0, n0);
     }
     if (p.zero_rest) {  // rows of no expert, a row to a warp
       const int end = min(max(__ldcg(p.offsets + p.experts), 0), p.M);
@@ -478,14 +668,14 @@ int tail_bytes(int bt, int experts) {
 }
 int stage_bytes(int bt) { return kWeightBytes + bt / 2 * kBlockK; }
 int stages_of(int bt, int experts) {
-  return std::min(kMaxStages, (kMaxDynamicSmem - 1024 - tail_bytes(bt, experts)) / stage_bytes(bt));
+  return std::min(bt == 64 ? kMaxStages : kWideStages, (kMaxDynamicSmem - 1024 - tail_bytes(bt, experts)) / stage_bytes(bt));
 }
 
-template <int CH>
+template <bool WIDE>
 cudaError_t launch(const GroupedParams& p, int pairs, int smem, const CUtensorMap& map_b, const CUtensorMap& map_big,
                    const CUtensorMap& map_small, cudaStream_t stream) {
   static OncePerDevice once;
-  const cudaError_t opted = once([] { return opt_in(fp8_grouped_kernel<CH>, kMaxDynamicSmem, false); });
+  const cudaError_t opted = once([] { return opt_in(fp8_grouped_kernel<WIDE>, kMaxDynamicSmem, false); });
   if (opted != cudaSuccess) return opted;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -501,14 +691,14 @@ cudaError_t launch(const GroupedParams& p, int pairs, int smem, const CUtensorMa
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, fp8_grouped_kernel<CH>, map_b, map_big, map_small, p);
+  return cudaLaunchKernelEx(&cfg, fp8_grouped_kernel<WIDE>, map_b, map_big, map_small, p);
 }
 
 }  // namespace
 
 int fp8_grouped_tile(int M, int experts) {
   const int mean = M / std::max(experts, 1);
-  return mean <= 48 ? 64 : mean <= 96 ? 128 : 256;
+  return mean <= 72 ? 64 : 256;
 }
 
 int fp8_grouped_smem(int tile, int experts) {
@@ -552,11 +742,8 @@ cudaError_t launch_fp8_grouped_gemm(const Fp8GroupedArgs& a, cudaStream_t stream
       !make_tensor_map(&map_small, a.a, (uint64_t)a.M, (uint64_t)a.K, 1, kSmallBox, kBlockK, 128))
     return cudaErrorInvalidValue;
   const int smem = fp8_grouped_smem(bt, a.experts);
-  switch (bt) {
-    case 64: return launch<1>(p, pairs, smem, map_b, map_big, map_small, stream);
-    case 128: return launch<2>(p, pairs, smem, map_b, map_big, map_small, stream);
-    default: return launch<4>(p, pairs, smem, map_b, map_big, map_small, stream);
-  }
+  return bt == 64 ? launch<false>(p, pairs, smem, map_b, map_big, map_small, stream)
+                  : launch<true>(p, pairs, smem, map_b, map_big, map_small, stream);
 }
 
 }  // namespace b200

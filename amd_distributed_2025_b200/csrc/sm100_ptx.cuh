@@ -202,12 +202,11 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&v)
       : "r"(taddr)
       : "memory");
 }
-// 16 lanes x 32 columns: thread i of the warp receives, of each group of 8 columns, columns 2 (i % 4) and the next of lanes
-// i / 4 (v[4 g], v[4 g + 1]) and i / 4 + 8 (v[4 g + 2], v[4 g + 3]).  The lane of the address is 0 or 16 in the warp's
-// quarter.
-__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&v)[16]) {
+// 16 lanes x 32 columns: thread i of the warp receives, of each group of 4 columns, column i % 4 of lanes i / 4 (v[2 g]) and
+// i / 4 + 8 (v[2 g + 1]).  The lane of the address is 0 or 16 in the warp's quarter.
+__device__ __forceinline__ void tmem_ld_16x128b_x8(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "tcgen05.ld.sync.aligned.16x128b.x8.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
