@@ -62,6 +62,21 @@ void check_no_gradient(const at::Tensor& t, const char* what) {
               " requires a gradient, and this operator has none: call it under torch.no_grad()");
 }
 
+// Two matrices of one shape and type, of which one is written while the other is read: the very same rows are fine (a lane
+// reads its columns before it writes them), and so are rows that do not meet.
+void check_apart_or_same(const at::Tensor& a, const at::Tensor& b, const char* what) {
+  if (a.numel() == 0 || (a.const_data_ptr() == b.const_data_ptr() && a.strides() == b.strides())) return;
+  const int64_t bytes = (int64_t)a.element_size(), rows = a.size(0), cols = a.size(1);
+  const auto reach = [&](const at::Tensor& t) { return ((rows - 1) * t.stride(0) + (cols - 1) * t.stride(1) + 1) * bytes; };
+  const int64_t apart = (int64_t)((intptr_t)a.const_data_ptr() - (intptr_t)b.const_data_ptr());
+  if (apart >= reach(b) || -apart >= reach(a)) return;
+  if (a.strides() == b.strides() && (cols == 1 || a.stride(1) == 1)) {  // columns of the same wider matrix
+    const int64_t step = a.stride(0) * bytes, within = ((apart % step) + step) % step;
+    if (within >= cols * bytes && within <= step - cols * bytes) return;
+  }
+  TORCH_CHECK(false, what, " overlap in memory and are not the same");
+}
+
 // (x, weight, eps, residual or None, total_out or None, normed) -> (q, scale, total or None, normed or None)
 PyObject* rms_norm_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&] {
@@ -98,9 +113,8 @@ PyObject* rms_norm_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (residual_in) check_device(*residual_in, x_in, "residual");
     if (total) {
       check_device(*total, x_in, "total_out");
-      // (the very same rows are fine: a lane reads its columns before it writes them)
-      at::assert_no_partial_overlap(*total, x_in);
-      at::assert_no_partial_overlap(*total, *residual_in);
+      check_apart_or_same(*total, x_in, "total_out and x");
+      check_apart_or_same(*total, *residual_in, "total_out and residual");
       at::assert_no_overlap(*total, weight_in);
     }
     c10::cuda::CUDAGuard guard(x_in.device());

@@ -7,11 +7,17 @@
 //
 // Everything is fp32 between the loads and the conversion.  The maximum carries NaN on (max.NaN), so that a block with a
 // NaN has a NaN for its scale and nothing but NaN in it; the floor of 1e-30 keeps the reciprocal of an empty block finite.
-// y is multiplied by the reciprocal of the scale, rounded once: a value within 2^-23 of the border between two e4m3 values
-// may fall to the other side of it than after a division.
+// y is multiplied by 448 over the maximum, from an approximate reciprocal (one step of fp32): a value that close to the
+// border between two e4m3 values may fall to the other side of it than after a division.
 //
-// A lane holds eight neighbouring columns of a block (sixteen lanes to a block) where rows are whole aligned 16-byte
-// vectors, else every 32nd column (a warp to a block): 2-byte loads and 1-byte stores of a warp stay neighbours.
+// A lane holds 16 neighbouring columns of a block (eight lanes to a block) where rows are whole aligned 32-byte pieces, eight
+// (sixteen lanes) where they are 16-byte pieces, else every 32nd column (a warp to a block), so that 2-byte loads and
+// 1-byte stores of a warp stay neighbours.
+//
+// Both are bound by memory where rows are whole pieces.  What that took is few instructions a value: blocks found by
+// eight lanes need three shuffles and one reciprocal for 16 values; with eight values to a lane, a division and four shuffles
+// for them, and the weight out of L2 for every row, 16384 x 4096 without a residual took as long as the memory takes
+// for 2.5 times the bytes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -19,6 +25,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_rows.h"
 #include "moe_common.cuh"
@@ -32,7 +39,8 @@ using moe::from_f32;
 using moe::to_f32;
 
 constexpr int kBlockCols = 128;
-constexpr int kNormThreads = 512;  // the most of a team: N = 8 vectors a lane leave 128 registers
+// The most lanes of a team: a row that has to be read value by value wants more of them.
+template <int PER> constexpr int kNormThreads = PER == 4 ? 1024 : 512;
 constexpr float kE4m3Max = 448.f;
 constexpr float kLeastMax = 1e-30f;
 
@@ -41,115 +49,162 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-
-__device__ __forceinline__ void unpack8(const int4& raw, float* f, __half) {
-  const __half2* h = reinterpret_cast<const __half2*>(&raw);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 v = __half22float2(h[j]);
-    f[2 * j] = v.x;
-    f[2 * j + 1] = v.y;
-  }
-}
-__device__ __forceinline__ void unpack8(const int4& raw, float* f, __nv_bfloat16) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 v = __bfloat1622float2(h[j]);
-    f[2 * j] = v.x;
-    f[2 * j + 1] = v.y;
-  }
-}
-
-// Eight values of T as they lie in memory.
-template <typename T> struct Raw8 { int4 v[sizeof(T) / 2]; };
-template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = __ldcg(reinterpret_cast<const int4*>(p) + i);
+__device__ __forceinline__ float warp_max_abs_nan(float a) {
+  float r;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(a));
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void to_floats(const Raw8<T>& r, float* f) {
-  if constexpr (sizeof(T) == 2) {
-    unpack8(r.v[0], f, T());
+__device__ __forceinline__ float reciprocal(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+
+// W words of 32 bits from or to global memory, A (4 or 8) at a time where there are as many: the address is a multiple of as
+// many bytes.
+template <int W, int A>
+__device__ __forceinline__ void load_words(uint32_t* w, const void* p) {
+  static_assert(W % 4 == 0, "pieces of 16 or 32 bytes");
+  if constexpr (W > A) {
+    load_words<A, A>(w, p);
+    load_words<W - A, A>(w + A, reinterpret_cast<const uint32_t*>(p) + A);
+  } else if constexpr (W == 8) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
   } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f[4 * i] = __int_as_float(r.v[i].x);
-      f[4 * i + 1] = __int_as_float(r.v[i].y);
-      f[4 * i + 2] = __int_as_float(r.v[i].z);
-      f[4 * i + 3] = __int_as_float(r.v[i].w);
-    }
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* f) {
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(p)[i] = moe::pack_vec<T>(f + i * (16 / (int)sizeof(T)));
+template <int W, int A>
+__device__ __forceinline__ void store_words(void* p, const uint32_t* w) {
+  if constexpr (W > A) {
+    store_words<A, A>(p, w);
+    store_words<W - A, A>(reinterpret_cast<uint32_t*>(p) + A, w + A);
+  } else if constexpr (W == 8) {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "l"(p)
+                 : "memory");
+  } else if constexpr (W == 4) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    static_assert(W == 2, "8, 16 or 32 bytes");
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
 }
 
-// How the columns of a row lie in the lanes.  A unit is what a lane has of a block: unit u of a team of lanes.
-template <bool VEC>
+__device__ __forceinline__ float2 two_floats(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 two_floats(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t two_packed(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t two_packed(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// How the columns of a row lie in the lanes.  A unit is what a lane has of a block: PER neighbouring columns (16 or 8), or, with
+// PER = 4, every 32nd.
+template <int PER>
 struct Lanes {
-  static constexpr int kPer = VEC ? 8 : 4;           // columns of a unit
-  static constexpr int kUnits = kBlockCols / kPer;   // lanes that share a block
-  // the first column of unit u, and of element e the distance from it
-  static __device__ __forceinline__ int64_t column(int u) {
-    return VEC ? (int64_t)u * 8 : (int64_t)(u >> 5) * kBlockCols + (u & 31);
-  }
-  static __device__ __forceinline__ int step(int e) { return VEC ? e : 32 * e; }
+  static constexpr bool kVec = PER != 4;
+  static constexpr int kUnits = kBlockCols / PER;  // lanes that share a block
+  static constexpr int kWords = PER / 2;           // of an access: addresses are multiples of 2 PER bytes
+  static __device__ __forceinline__ int column(int u) { return kVec ? u * PER : (u >> 5) * kBlockCols + (u & 31); }
 
+  // A unit as it lies in memory.
+  template <typename T> struct Raw { uint32_t w[kVec ? PER * (int)sizeof(T) / 4 : PER]; };
+
+  // (columns behind the row are zeros)
   template <typename T>
-  static __device__ __forceinline__ void load(const T* row, int u, int cols, float* f) {
-    const int64_t c = column(u);
-    if constexpr (VEC) {
+  static __device__ __forceinline__ Raw<T> load(const T* row, int u, int cols) {
+    Raw<T> r;
+    const int c = column(u);
+    if constexpr (kVec) {
       if (c < cols) {
-        to_floats<T>(load8<T>(row + c), f);
+        load_words<PER * (int)sizeof(T) / 4, kWords>(r.w, row + c);
       } else {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) f[e] = 0.f;
+        for (int i = 0; i < PER * (int)sizeof(T) / 4; ++i) r.w[i] = 0;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) f[e] = c + step(e) < cols ? to_f32(row[c + step(e)]) : 0.f;
+      for (int e = 0; e < PER; ++e) r.w[e] = c + 32 * e < cols ? bits(row[c + 32 * e]) : 0u;
+    }
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
+  static __device__ __forceinline__ uint32_t bits(__half v) { return __half_as_ushort(v); }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+
+  template <typename T>
+  static __device__ __forceinline__ void floats(const Raw<T>& r, float* f) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if constexpr (sizeof(T) == 4) {
+        f[e] = __uint_as_float(r.w[e]);
+      } else if constexpr (kVec) {
+        if (e % 2 == 0) {
+          const float2 v = two_floats(r.w[e / 2], T());
+          f[e] = v.x;
+          f[e + 1] = v.y;
+        }
+      } else {
+        f[e] = two_floats(r.w[e], T()).x;
+      }
     }
   }
   template <typename T>
   static __device__ __forceinline__ void store(T* row, int u, int cols, const float* f) {
-    const int64_t c = column(u);
-    if constexpr (VEC) {
-      if (c < cols) store8<T>(row + c, f);
+    const int c = column(u);
+    if constexpr (kVec) {
+      if (c >= cols) return;
+      uint32_t w[PER * (int)sizeof(T) / 4];
+#pragma unroll
+      for (int i = 0; i < PER * (int)sizeof(T) / 4; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+        else w[i] = two_packed(f[2 * i], f[2 * i + 1], T());
+      }
+      store_words<PER * (int)sizeof(T) / 4, kWords>(row + c, w);
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (c + step(e) < cols) row[c + step(e)] = from_f32<T>(f[e]);
+      for (int e = 0; e < PER; ++e)
+        if (c + 32 * e < cols) row[c + 32 * e] = from_f32<T>(f[e]);
     }
   }
   // Block scale and e4m3 values of one unit (every lane of the warp takes part; columns behind the row hold zeros).
   static __device__ __forceinline__ void quantise(uint8_t* q_row, float* scale_row, int u, int cols, const float* y) {
     float most = fabsf(y[0]);
 #pragma unroll
-    for (int e = 1; e < kPer; ++e) most = max_nan(most, fabsf(y[e]));
-#pragma unroll
-    for (int o = kUnits / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float scale = __fdiv_rn(max_nan(most, kLeastMax), kE4m3Max);
-    const float inverse = __frcp_rn(scale);
-    const int64_t c = column(u);
-    if (c >= cols) return;
-    if (u % kUnits == 0) scale_row[u / kUnits] = scale;
-    if constexpr (VEC) {
-      uint2 packed;
-      uint16_t* half = reinterpret_cast<uint16_t*>(&packed);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        half[e] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * e] * inverse, y[2 * e + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<uint2*>(q_row + c) = packed;
+    for (int e = 1; e < PER; ++e) most = max_nan(most, fabsf(y[e]));
+    if constexpr (kUnits == 32) {
+      most = warp_max_abs_nan(most);
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (c + step(e) < cols) q_row[c + step(e)] = __nv_cvt_float_to_fp8(y[e] * inverse, __NV_SATFINITE, __NV_E4M3);
+      for (int o = kUnits / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    most = max_nan(most, kLeastMax);
+    const float inverse = kE4m3Max * reciprocal(most);
+    const int c = column(u);
+    if (c >= cols) return;
+    if (u % kUnits == 0) scale_row[u / kUnits] = most * (1.f / kE4m3Max);
+    if constexpr (kVec) {
+      uint32_t packed[PER / 4];
+#pragma unroll
+      for (int i = 0; i < PER / 4; ++i) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * i] * inverse, y[4 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi =
+            __nv_cvt_float2_to_fp8x2(make_float2(y[4 * i + 2] * inverse, y[4 * i + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
+        packed[i] = lo | hi << 16;
+      }
+      store_words<PER / 4, kWords>(q_row + c, packed);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (c + 32 * e < cols) q_row[c + 32 * e] = __nv_cvt_float_to_fp8(y[e] * inverse, __NV_SATFINITE, __NV_E4M3);
     }
   }
 };
@@ -157,69 +212,87 @@ struct Lanes {
 }  // namespace
 
 // A team of blockDim.x lanes takes a row and keeps it in registers, N units a lane: it is read once.  With blockDim.y > 1
-// (short rows) a team is a warp, and the CTA has several.
-template <typename T, typename W, bool VEC, int N>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_fp8_kernel(const RmsNormFp8Args p) {
-  using L = Lanes<VEC>;
-  __shared__ float sums[32];
-  const int lanes = (int)blockDim.x;
+// (short rows) a team is a warp, and the CTA has several.  Teams go from row to row, four times as many as are resident at once:
+// that evens out what a few of them lose on memory.  16384 x 4096 bf16 with residual, us: a row to a CTA 108; from row to row,
+// the next one under way 81, with the weight out of L1 instead of registers 79, teams as many as are resident 83, four times as
+// many 73; without the next one under way 92; a warp to a row 152.
+template <typename T, typename W, int PER, int N>
+__global__ void __launch_bounds__(kNormThreads<PER>, N == 1 && sizeof(T) == 2 && PER > 4 ? 2 : 1) rms_norm_fp8_kernel(const RmsNormFp8Args p) {
+  using L = Lanes<PER>;
+  using RawT = typename L::template Raw<T>;
+  __shared__ float sums[2][32];
+  const int lanes = (int)blockDim.x, u0 = (int)threadIdx.x;
   const int blocks = (p.cols + kBlockCols - 1) / kBlockCols;
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows; row += (int64_t)gridDim.x * blockDim.y) {
-    float h[N][L::kPer];
-    const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
+  if (row >= p.rows) return;  // (a whole warp, and where a team is more than one, a whole CTA)
+  const T* const xs = reinterpret_cast<const T*>(p.x);
+  const T* const rs = reinterpret_cast<const T*>(p.residual);
+  // Up to two units a lane: the next row is on its way while this one is worked on.
+  constexpr bool kAhead = N <= 2;
+  constexpr int kKept = kAhead ? N : 1;
+  RawT x[kKept], r[kKept];
+  auto load_row = [&](int64_t at) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) L::load(x, i * lanes + (int)threadIdx.x, p.cols, h[i]);
-    if (p.residual != nullptr) {
-      const T* r = reinterpret_cast<const T*>(p.residual) + row * p.residual_stride;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float f[L::kPer];
-        L::load(r, i * lanes + (int)threadIdx.x, p.cols, f);
-#pragma unroll
-        for (int e = 0; e < L::kPer; ++e) h[i][e] += f[e];
-      }
+    for (int i = 0; i < kKept; ++i) {
+      x[i] = L::load(xs + at * p.x_stride, i * lanes + u0, p.cols);
+      if (p.residual != nullptr) r[i] = L::load(rs + at * p.residual_stride, i * lanes + u0, p.cols);
     }
+  };
+  if (kAhead) load_row(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    float h[N][PER];
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+      const int u = i * lanes + u0;
+      L::floats(kAhead ? x[i % kKept] : L::load(xs + row * p.x_stride, u, p.cols), h[i]);
+      if (p.residual != nullptr) {
+        float f[PER];
+        L::floats(kAhead ? r[i % kKept] : L::load(rs + row * p.residual_stride, u, p.cols), f);
 #pragma unroll
-      for (int e = 0; e < L::kPer; ++e) sum = fmaf(h[i][e], h[i][e], sum);
+        for (int e = 0; e < PER; ++e) h[i][e] += f[e];
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lanes > 32) {  // (a CTA with a team of several warps has one team)
-      if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
-      __syncthreads();
-      sum = (int)(threadIdx.x & 31) < lanes / 32 ? sums[threadIdx.x & 31] : 0.f;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      __syncthreads();
+      for (int e = 0; e < PER; ++e) sum = fmaf(h[i][e], h[i][e], sum);
     }
+    // (total may be x or residual: a lane has read its columns of this row, and nobody else reads them)
     if (p.total != nullptr) {
       T* total = reinterpret_cast<T*>(p.total) + row * p.total_stride;
 #pragma unroll
-      for (int i = 0; i < N; ++i) L::store(total, i * lanes + (int)threadIdx.x, p.cols, h[i]);
+      for (int i = 0; i < N; ++i) L::store(total, i * lanes + u0, p.cols, h[i]);
+    }
+    if (kAhead && row + step < p.rows) load_row(row + step);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lanes > 32) {  // (a CTA with a team of several warps has one team; rows take turns with the two sets of sums)
+      if ((u0 & 31) == 0) sums[turn][u0 >> 5] = sum;
+      __syncthreads();
+      sum = (u0 & 31) < lanes / 32 ? sums[turn][u0 & 31] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     const float rstd = rsqrtf(sum / (float)p.cols + p.eps);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int u = i * lanes + (int)threadIdx.x;
-      float w[L::kPer];
-      L::load(reinterpret_cast<const W*>(p.weight), u, p.cols, w);
+      const int u = i * lanes + u0;
+      float f[PER];
+      L::floats(L::load(reinterpret_cast<const W*>(p.weight), u, p.cols), f);  // (out of L1)
 #pragma unroll
-      for (int e = 0; e < L::kPer; ++e) h[i][e] = h[i][e] * rstd * w[e];
+      for (int e = 0; e < PER; ++e) h[i][e] = h[i][e] * rstd * f[e];
       if (p.normed != nullptr) L::store(reinterpret_cast<T*>(p.normed) + row * p.cols, u, p.cols, h[i]);
       L::quantise(reinterpret_cast<uint8_t*>(p.q) + row * p.cols, p.scale + row * blocks, u, p.cols, h[i]);
     }
   }
 }
 
-// A team of blockDim.x lanes takes a row, a unit a lane at a time; a CTA has blockDim.y teams.  Teams are whole warps, or
-// (vectors only) halves of one.
-template <typename T, bool VEC>
+// A team of blockDim.x lanes takes a row, a unit a lane at a time; a CTA has blockDim.y teams.  Teams are whole warps, or parts
+// of one that hold whole blocks.
+template <typename T, int PER>
 __global__ void __launch_bounds__(256) silu_mul_fp8_kernel(const SiluMulFp8Args p) {
-  using L = Lanes<VEC>;
+  using L = Lanes<PER>;
   const int lanes = (int)blockDim.x;
   const int blocks = (p.cols + kBlockCols - 1) / kBlockCols;
   ptx::grid_dep_launch();
@@ -230,11 +303,12 @@ __global__ void __launch_bounds__(256) silu_mul_fp8_kernel(const SiluMulFp8Args 
     const int cols = row < p.rows ? p.cols : 0;
     const T* gate = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
     for (int u = (int)threadIdx.x; u < blocks * L::kUnits; u += lanes) {
-      float g[L::kPer], v[L::kPer];
-      L::load(gate, u, cols, g);
-      L::load(gate + p.cols, u, cols, v);
+      const auto rg = L::load(gate, u, cols), ru = L::load(gate + p.cols, u, cols);
+      float g[PER], v[PER];
+      L::floats(rg, g);
+      L::floats(ru, v);
 #pragma unroll
-      for (int e = 0; e < L::kPer; ++e) g[e] = __fdividef(g[e], 1.f + __expf(-g[e])) * v[e];
+      for (int e = 0; e < PER; ++e) g[e] = __fdividef(g[e], 1.f + __expf(-g[e])) * v[e];
       L::quantise(reinterpret_cast<uint8_t*>(p.q) + row * p.cols, p.scale + row * blocks, u, cols, g);
     }
   }
@@ -244,8 +318,6 @@ __global__ void __launch_bounds__(256) silu_mul_fp8_kernel(const SiluMulFp8Args 
 // host side
 // ---------------------------------------------------------------------------------------
 namespace {
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename P>
 cudaError_t launch_teams(void (*kernel)(P), int64_t grid, dim3 block, cudaStream_t stream, const P& p) {
@@ -261,34 +333,51 @@ cudaError_t launch_teams(void (*kernel)(P), int64_t grid, dim3 block, cudaStream
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <typename T, typename W, bool VEC>
+// Columns of a unit, from everything that has to be a multiple of it: sizes and strides in elements, addresses in bytes.
+int columns_of_a_unit(int64_t elements, uint64_t addresses) {
+  if (elements % 16 == 0 && addresses % 32 == 0) return 16;
+  return elements % 8 == 0 && addresses % 16 == 0 ? 8 : 4;
+}
+uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+template <typename T, typename W, int PER>
 cudaError_t norm_units(const RmsNormFp8Args& p, int sms, cudaStream_t stream) {
-  const int units = (p.cols + kBlockCols - 1) / kBlockCols * Lanes<VEC>::kUnits;
-  constexpr int kShort = 4 * 32;  // units of a row that one warp takes
+  const int units = (p.cols + kBlockCols - 1) / kBlockCols * Lanes<PER>::kUnits;
   dim3 block;
   int n;
-  if (units <= kShort) {
+  if (units <= 64) {
     n = (units + 31) / 32;
     block = dim3(32, 8);
   } else {
-    n = std::max(2, (units + kNormThreads - 1) / kNormThreads);
+    n = (units + kNormThreads<PER> - 1) / kNormThreads<PER>;
     block = dim3((unsigned)(((units + n - 1) / n + 31) / 32 * 32), 1);
   }
-  const int64_t grid = std::min<int64_t>((p.rows + block.y - 1) / block.y, 1 << 30);
-  auto go = [&](auto kernel) { return launch_teams(kernel, grid, block, stream, p); };
-  if (n <= 1) return go(rms_norm_fp8_kernel<T, W, VEC, 1>);
-  if (n <= 2) return go(rms_norm_fp8_kernel<T, W, VEC, 2>);
-  if (n <= 4) return go(rms_norm_fp8_kernel<T, W, VEC, 4>);
-  if (n <= 8) return go(rms_norm_fp8_kernel<T, W, VEC, 8>);
-  if constexpr (!VEC) return go(rms_norm_fp8_kernel<T, W, VEC, 16>);
+  const int64_t teams = (p.rows + block.y - 1) / block.y;
+  const int threads = (int)(block.x * block.y);
+  const auto go = [&](auto n_units) {
+    constexpr auto kernel = rms_norm_fp8_kernel<T, W, PER, decltype(n_units)::value>;
+    static thread_local int known[kNormThreads<PER> / 32 + 1] = {};  // CTAs that an SM holds, by their size
+    int& ctas = known[threads / 32];
+    if (ctas == 0 && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, 0) != cudaSuccess) ctas = 1;
+    return launch_teams(kernel, std::min<int64_t>(teams, 4 * (int64_t)sms * std::max(ctas, 1)), block, stream, p);
+  };
+  if (n <= 1) return go(std::integral_constant<int, 1>());
+  if (n <= 2) return go(std::integral_constant<int, 2>());
+  if (n <= 4) return go(std::integral_constant<int, 4>());
+  if constexpr (PER <= 8) {
+    if (n <= 8) return go(std::integral_constant<int, 8>());
+  }
   return cudaErrorInvalidValue;
 }
 
 template <typename T, typename W>
 cudaError_t norm_typed(const RmsNormFp8Args& p, int sms, cudaStream_t stream) {
-  const bool vec = p.cols % 8 == 0 && p.x_stride % 8 == 0 && p.residual_stride % 8 == 0 && p.total_stride % 8 == 0 &&
-                   aligned16(p.x) && aligned16(p.residual) && aligned16(p.weight) && aligned16(p.total);
-  return vec ? norm_units<T, W, true>(p, sms, stream) : norm_units<T, W, false>(p, sms, stream);
+  switch (columns_of_a_unit(p.cols | p.x_stride | p.residual_stride | p.total_stride,
+                            address(p.x) | address(p.residual) | address(p.weight) | address(p.total))) {
+    case 16: return norm_units<T, W, 16>(p, sms, stream);
+    case 8: return norm_units<T, W, 8>(p, sms, stream);
+    default: return norm_units<T, W, 4>(p, sms, stream);
+  }
 }
 
 template <typename T>
@@ -297,19 +386,25 @@ cudaError_t norm_weight(const RmsNormFp8Args& p, int sms, cudaStream_t stream) {
   return p.weight_dtype == 2 ? norm_typed<T, float>(p, sms, stream) : cudaErrorInvalidValue;
 }
 
-template <typename T>
-cudaError_t silu_typed(const SiluMulFp8Args& p, int sms, cudaStream_t stream) {
-  const bool vec = p.cols % 8 == 0 && p.x_stride % 8 == 0 && aligned16(p.x);
-  const int units = (p.cols + kBlockCols - 1) / kBlockCols * (vec ? 16 : 32);
-  // the largest team of which the least is idle in the last round
-  int lanes = 32;
-  for (int l = 64; l <= 256; l *= 2)
-    if ((units + l - 1) / l * l <= (units + lanes - 1) / lanes * lanes) lanes = l;
-  if (units <= 16) lanes = 16;
+template <typename T, int PER>
+cudaError_t silu_units(const SiluMulFp8Args& p, int sms, cudaStream_t stream) {
+  const int units = (p.cols + kBlockCols - 1) / kBlockCols * Lanes<PER>::kUnits;
+  // the largest team of which no more than a ninth is idle
+  int lanes = Lanes<PER>::kUnits;
+  for (int l = 2 * lanes; l <= 256; l *= 2)
+    if (8 * ((units + l - 1) / l * l) <= 9 * units) lanes = l;
   const dim3 block((unsigned)lanes, (unsigned)(256 / lanes));
   const int64_t grid = std::min<int64_t>((p.rows + block.y - 1) / block.y, 1 << 30);
-  return vec ? launch_teams(silu_mul_fp8_kernel<T, true>, grid, block, stream, p)
-             : launch_teams(silu_mul_fp8_kernel<T, false>, grid, block, stream, p);
+  return launch_teams(silu_mul_fp8_kernel<T, PER>, grid, block, stream, p);
+}
+
+template <typename T>
+cudaError_t silu_typed(const SiluMulFp8Args& p, int sms, cudaStream_t stream) {
+  switch (columns_of_a_unit(p.cols | p.x_stride, address(p.x))) {
+    case 16: return silu_units<T, 16>(p, sms, stream);
+    case 8: return silu_units<T, 8>(p, sms, stream);
+    default: return silu_units<T, 4>(p, sms, stream);
+  }
 }
 
 }  // namespace

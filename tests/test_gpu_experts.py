@@ -123,6 +123,23 @@ def test_rms_norm_fp8_weight_in_fp32_strides_and_alignment():
     _check_norm(wide[:, :512], shifted, None, rms_norm_fp8(wide[:, :512], shifted))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_fp8_rows_at_every_alignment(dtype):
+    """Rows and weights that begin 0, 8, 16, .. bytes and single elements behind a 32-byte border, with distances to match."""
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8, silu_mul_fp8
+
+    step = 8 // torch.tensor([], dtype=dtype).element_size()
+    for cols in (256, 264, 2048):
+        wide, other = _randn(5, cols + 80, dtype=dtype, seed=1), _randn(5, 2 * cols + 96, dtype=dtype, seed=2)
+        long = 1 + 0.1 * _randn(cols + 80, seed=3)
+        for lo in (0, step, 2 * step, 3 * step, 4 * step, 1):
+            x, r = wide[:, lo:lo + cols], other[:, lo:lo + cols]
+            for w in (long.to(dtype)[lo:lo + cols], long[lo:lo + cols]):
+                _check_norm(x, w, r, rms_norm_fp8(x, w, residual=r, normed=True))
+            x = other[:, lo:lo + 2 * cols]
+            _check_silu(x, silu_mul_fp8(x))
+
+
 @pytest.mark.parametrize("cols", [1024, 1500, 4100])
 def test_rms_norm_fp8_total_in_place(cols):
     from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
@@ -141,8 +158,15 @@ def test_rms_norm_fp8_total_in_place(cols):
     assert torch.equal(room[:, 8:8 + cols], want.total)
     assert bool((room[:, :8] == 7).all()) and bool((room[:, 8 + cols:] == 7).all())
     both = torch.zeros(41, cols, dtype=torch.bfloat16, device="cuda")
-    with pytest.raises(RuntimeError, match="overlap|memory location"):
-        rms_norm_fp8(both[:40], w, residual=r, total_out=both[1:])
+    for bad in (lambda: rms_norm_fp8(both[:40], w, residual=r, total_out=both[1:]),
+                lambda: rms_norm_fp8(r, w, residual=both[:40], total_out=both[1:]),
+                lambda: rms_norm_fp8(both[:1].expand(40, cols), w, residual=r, total_out=both[:40])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            bad()
+    side = torch.zeros(40, 2 * cols + 8, dtype=torch.bfloat16, device="cuda")  # the sum beside its residual
+    side[:, :cols] = r
+    rms_norm_fp8(x, w, residual=side[:, :cols], total_out=side[:, cols + 8:])
+    assert torch.equal(side[:, cols + 8:], want.total) and torch.equal(side[:, :cols], r)
 
 
 def test_rms_norm_fp8_zeros_infinities_and_nan():
