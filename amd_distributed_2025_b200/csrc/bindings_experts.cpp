@@ -57,8 +57,10 @@ at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Tensor
 
 // ------------------------------------------------------------- rows with block scales ----
 
+bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+
 void check_no_gradient(const at::Tensor& t, const char* what) {
-  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), what,
+  TORCH_CHECK(!wants_gradient(t), what,
               " requires a gradient, and this operator has none: call it under torch.no_grad()");
 }
 
@@ -187,11 +189,13 @@ int64_t check_entries(int64_t tokens, int64_t k) {
   return tokens * k;
 }
 
-// (x, indices, num_experts, scale or None) -> (rows, rows_scale or None, offsets, row_of)
+
+// (x, indices, num_experts, scale or None) -> (rows, rows_scale or None, offsets, row_of); None where x wants a gradient
 PyObject* sort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded([&] {
+  return guarded([&]() -> PyObject* {
     count_args(n, 4);
     const at::Tensor& x_in = tensor_arg(v[0]);
+    if (wants_gradient(x_in)) Py_RETURN_NONE;
     const at::Tensor& indices_in = tensor_arg(v[1]);
     const int64_t experts = int_arg(v[2]);
     const optional<at::Tensor> scale_in = optional_arg(v[3]);
@@ -258,13 +262,15 @@ at::Tensor weights_of(const at::Tensor& w, const at::Tensor& row_of) {
   return w;
 }
 
-// (rows, row_of, weights or None) -> out
+// (rows, row_of, weights or None) -> out; None where something wants a gradient, or weights are of another type
 PyObject* unsort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded([&] {
+  return guarded([&]() -> PyObject* {
     count_args(n, 3);
     const at::Tensor& rows_in = tensor_arg(v[0]);
     const at::Tensor& row_of_in = tensor_arg(v[1]);
     const optional<at::Tensor> weights_in = optional_arg(v[2]);
+    if (wants_gradient(rows_in) || (weights_in && (wants_gradient(*weights_in) || weights_in->scalar_type() != at::kFloat)))
+      Py_RETURN_NONE;
     TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(1) >= 1 && rows_in.size(1) <= INT32_MAX / 8, "rows must be a matrix [rows, hidden]");
     const int code = dtype_code(rows_in.scalar_type());
     check_order(row_of_in, "row_of");
@@ -467,5 +473,6 @@ void b200::bind_experts(py::module& m) {
   if (PyModule_AddFunctions(m.ptr(), kExpertCalls) != 0) throw py::error_already_set();
   m.def("adds_up_elsewhere", &adds_up_elsewhere);
   m.def("fp8_grouped_tile", &b200::fp8_grouped_tile);
+  m.def("fp8_grouped_local_bytes", &b200::fp8_grouped_local_bytes);
   m.def("fp8_grouped_share", [](int tile, int experts) { return py::make_tuple(b200::fp8_grouped_smem(tile, experts), 512); });
 }

@@ -52,6 +52,8 @@ constexpr int kGroupedMaxExperts = 1024;  // their tables lie in shared memory
 // Tokens of a tile as planned for a problem, and the shared memory of a CTA with such tiles (for tests).
 int fp8_grouped_tile(int M, int experts);
 int fp8_grouped_smem(int tile, int experts);
+// Local memory of a thread: anything but 0 is registers that did not suffice, in the loop as a rule.
+int fp8_grouped_local_bytes(int tile);
 cudaError_t launch_fp8_grouped_gemm(const Fp8GroupedArgs& args, cudaStream_t stream);
 
 // Self-test of the bounded wait: one warp waits for a barrier that nothing signals and leaves its record.

@@ -331,18 +331,18 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
 #pragma unroll
               for (int i = 0; i < kGroup; ++i) s[c][i] = 0.f;
             } else if (p.vec_scales) {
-              const float4 f = *reinterpret_cast<const float4*>(as + kb);
+              const float4 f = __ldca(reinterpret_cast<const float4*>(as + kb));
               s[c][0] = f.x, s[c][1] = f.y, s[c][2] = f.z, s[c][3] = f.w;
             } else {
 #pragma unroll
-              for (int i = 0; i < kGroup; ++i) s[c][i] = as[min(kb + i, p.k_blocks - 1) * p.as_stride_k];
+              for (int i = 0; i < kGroup; ++i) s[c][i] = __ldca(as + min(kb + i, p.k_blocks - 1) * p.as_stride_k);
             }
           }
           float b[2][kGroup];
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
-            b[0][i] = b0[min(kb + i, p.k_blocks - 1) * p.bs_stride_k];
-            if (WIDE) b[1][i] = b1[min(kb + i, p.k_blocks - 1) * p.bs_stride_k];
+            b[0][i] = __ldca(b0 + min(kb + i, p.k_blocks - 1) * p.bs_stride_k);
+            if (WIDE) b[1][i] = __ldca(b1 + min(kb + i, p.k_blocks - 1) * p.bs_stride_k);
           }
           if (!fp8_wait(sempty_bar(slot), phase ^ 1u, &abort_flag, p, 500 + (int)slot)) break;
           const uint32_t at = scales + slot * kSlotBytes;
@@ -703,6 +703,12 @@ int fp8_grouped_tile(int M, int experts) {
 
 int fp8_grouped_smem(int tile, int experts) {
   return 1024 + stages_of(tile, experts) * stage_bytes(tile) + tail_bytes(tile, experts);
+}
+
+int fp8_grouped_local_bytes(int tile) {
+  cudaFuncAttributes a = {};
+  const cudaError_t e = tile == 64 ? cudaFuncGetAttributes(&a, fp8_grouped_kernel<false>) : cudaFuncGetAttributes(&a, fp8_grouped_kernel<true>);
+  return e == cudaSuccess ? (int)a.localSizeBytes : -1;
 }
 
 cudaError_t launch_fp8_grouped_gemm(const Fp8GroupedArgs& a, cudaStream_t stream) {

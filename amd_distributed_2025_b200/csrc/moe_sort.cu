@@ -31,22 +31,55 @@ namespace {
 using namespace moe;
 
 // Copies move vectors V, U of them a lane at a time: the widest that rows, their distance and their addresses allow.
-template <typename V> struct Copy { static constexpr int U = sizeof(V) == 16 ? 2 : sizeof(V) == 4 ? 4 : 8; };
+struct Vec32 { uint32_t w[8]; };
+template <typename V> struct Copy {
+  static constexpr int U = sizeof(V) == 32 ? 1 : sizeof(V) == 16 ? 2 : sizeof(V) == 4 ? 4 : 8;
+};
+template <typename V>
+__device__ __forceinline__ V load_vec(const V* p) { return __ldcg(p); }
+template <>
+__device__ __forceinline__ Vec32 load_vec<Vec32>(const Vec32* p) {
+  Vec32 v;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p));
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ void store_vec(V* p, const V& v) { *p = v; }
+template <>
+__device__ __forceinline__ void store_vec<Vec32>(Vec32* p, const Vec32& v) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]),
+               "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7]), "l"(p)
+               : "memory");
+}
 
 struct SortParams {
   SortTokensArgs a;
   int32_t pieces;      // of a row; the scales are one more
   int32_t row_vecs, piece_vecs;
-  int32_t chunks, chunk_tokens, ctas_of_chunk;  // two launches: runs of tokens that are counted by a CTA each
+  int32_t vec_ids;               // 1: ids begin at a multiple of 16 bytes
+  int32_t chunks, chunk_tokens;  // two launches: runs of tokens that are counted by a CTA each
 };
 
+__device__ __forceinline__ int checked_id(long long e, int experts) { return e >= 0 && e < experts ? (int)e : -1; }
 __device__ __forceinline__ int expert_of(const SortTokensArgs& a, int64_t i) {
+  return checked_id(a.wide_ids ? __ldcg(reinterpret_cast<const long long*>(a.indices) + i)
+                               : (long long)__ldcg(reinterpret_cast<const int*>(a.indices) + i),
+                    a.experts);
+}
+// Entries 4 q .. 4 q + 3, from aligned ids.
+__device__ __forceinline__ void experts_of(const SortTokensArgs& a, int q, int (&e)[4]) {
   if (a.wide_ids) {
-    const long long e = __ldcg(reinterpret_cast<const long long*>(a.indices) + i);
-    return e >= 0 && e < a.experts ? (int)e : -1;
+    const longlong2* ids = reinterpret_cast<const longlong2*>(a.indices) + 2 * (int64_t)q;
+    const longlong2 u = __ldcg(ids), v = __ldcg(ids + 1);
+    e[0] = checked_id(u.x, a.experts), e[1] = checked_id(u.y, a.experts);
+    e[2] = checked_id(v.x, a.experts), e[3] = checked_id(v.y, a.experts);
+  } else {
+    const int4 u = __ldcg(reinterpret_cast<const int4*>(a.indices) + q);
+    e[0] = checked_id(u.x, a.experts), e[1] = checked_id(u.y, a.experts);
+    e[2] = checked_id(u.z, a.experts), e[3] = checked_id(u.w, a.experts);
   }
-  const int e = __ldcg(reinterpret_cast<const int*>(a.indices) + i);
-  return e >= 0 && e < a.experts ? e : -1;
 }
 
 // counts[0 .. n) in shared memory become exclusive prefix sums; returns their total.  All threads of the CTA.
@@ -79,36 +112,49 @@ __device__ __forceinline__ int exclusive_scan(int32_t* counts, int n, int32_t* w
   return total;
 }
 
-// One piece of token t's row (or, behind the last piece, its scales) to its k rows; `row` is lane j's: entry j's row.
+// One piece of token t's row: a warp asks for it ...
 template <typename V>
-__device__ __forceinline__ void copy_piece(const SortParams& p, int t, int piece, int row) {
+__device__ __forceinline__ void load_piece(const SortParams& p, int t, int piece, V* r) {
+  constexpr int U = Copy<V>::U;
+  const V* src = reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(p.a.x) + (int64_t)t * p.a.x_stride);
+  const int v0 = piece * p.piece_vecs + (int)(threadIdx.x & 31);
+  const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (v0 + 32 * u < v1) r[u] = load_vec(src + v0 + 32 * u);
+}
+// ... and stores it to the token's k rows; `row` is lane j's: entry j's row.  (Behind the last piece: the token's scales.)
+template <typename V>
+__device__ __forceinline__ void store_piece(const SortParams& p, int t, int piece, int row, const V* r) {
   constexpr int U = Copy<V>::U;
   const int lane = threadIdx.x & 31;
   const SortTokensArgs& a = p.a;
   if (piece < p.pieces) {
-    const V* src = reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(a.x) + (int64_t)t * a.x_stride);
     const int v0 = piece * p.piece_vecs + lane;
     const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
-    V r[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + 32 * u < v1) r[u] = __ldcg(src + v0 + 32 * u);
     for (int j = 0; j < a.k; ++j) {
       const int to = __shfl_sync(0xffffffffu, row, j);
       if (to < 0) continue;
       V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(a.rows) + (int64_t)to * a.row_bytes);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (v0 + 32 * u < v1) dst[v0 + 32 * u] = r[u];
+        if (v0 + 32 * u < v1) store_vec(dst + v0 + 32 * u, r[u]);
     }
   } else {
+    // A row's scales are no whole number of cache lines, and its neighbours' come at another time: lines that are written in
+    // parts stay in L2 until they are complete (65536 rows of 224 bytes: 126 us -> SCALEUS).
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
     const float* src = a.scale + (int64_t)t * a.scale_stride;
     for (int c0 = 0; c0 < a.scale_cols; c0 += 32) {
       const bool in = c0 + lane < a.scale_cols;
       const float s = in ? __ldcg(src + c0 + lane) : 0.f;
       for (int j = 0; j < a.k; ++j) {
         const int to = __shfl_sync(0xffffffffu, row, j);
-        if (to >= 0 && in) a.rows_scale[(int64_t)to * a.scale_cols + c0 + lane] = s;
+        if (to >= 0 && in)
+          asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(a.rows_scale + (int64_t)to * a.scale_cols + c0 + lane),
+                       "f"(s), "l"(policy)
+                       : "memory");
       }
     }
   }
@@ -118,10 +164,10 @@ __device__ __forceinline__ void copy_piece(const SortParams& p, int t, int piece
 template <typename V>
 __device__ __forceinline__ void zero_rows(void* rows, int64_t row_bytes, float* scales, int scale_cols, int64_t from, int64_t to,
                                           int cta, int ctas) {
-  const V zero = V();
+  const V zero = {};
   for (int64_t r = from + cta; r < to; r += ctas) {
     V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(rows) + r * row_bytes);
-    for (int v = threadIdx.x; v < (int)(row_bytes / (int64_t)sizeof(V)); v += blockDim.x) dst[v] = zero;
+    for (int v = threadIdx.x; v < (int)(row_bytes / (int64_t)sizeof(V)); v += blockDim.x) store_vec(dst + v, zero);
     if (scales != nullptr)
       for (int c = threadIdx.x; c < scale_cols; c += blockDim.x) scales[r * scale_cols + c] = 0.f;
   }
@@ -131,8 +177,8 @@ __device__ __forceinline__ void zero_rows(void* rows, int64_t row_bytes, float* 
 
 // One launch: every CTA counts all entries itself, and ranks its own against each other.
 template <typename V>
-__global__ void __launch_bounds__(512) sort_tokens_kernel(const SortParams p) {
-  extern __shared__ int32_t smem[];
+__global__ void __launch_bounds__(1024) sort_tokens_kernel(const SortParams p) {
+  extern __shared__ __align__(16) int32_t smem[];
   __shared__ int32_t warp_sums[32];
   const SortTokensArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x;
@@ -141,21 +187,34 @@ __global__ void __launch_bounds__(512) sort_tokens_kernel(const SortParams p) {
   const int lo = (int)(items * blockIdx.x / gridDim.x), hi = (int)(items * (blockIdx.x + 1) / gridDim.x);
   const int t0 = lo / P, t1 = hi > lo ? (hi + P - 1) / P : t0;
   const int i0 = t0 * a.k, i1 = t1 * a.k, n = a.tokens * a.k;
-  int32_t* start = smem;                // entries of all of an expert, then the first row of each
-  int32_t* before = start + a.experts;  // own entries and earlier ones
-  int32_t* ids = before + a.experts;    // expert of each own entry, then its row
-  for (int e = tid; e < 2 * a.experts; e += threads) smem[e] = 0;
+  int32_t* start = smem;  // entries of an expert behind the CTA's, then all of them, then the first row
+  const int room = (a.experts + 3) & ~3, own = (i1 - i0 + 3) & ~3;
+  int32_t* before = start + room;  // own entries and earlier ones
+  int32_t* ids = before + room;    // expert of each own entry
+  int32_t* rows = ids + own;       // and its row
+  for (int e = tid; e < 2 * room; e += threads) smem[e] = 0;
+  if (tid < own - (i1 - i0)) ids[i1 - i0 + tid] = -2;
   __syncthreads();
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  for (int i = tid; i < n; i += threads) {
-    const int e = expert_of(a, i);
-    if (e >= 0) {
-      atomicAdd(start + e, 1);
-      if (i < i1) atomicAdd(before + e, 1);
-    }
+  int item = lo + (tid >> 5);
+  V first[Copy<V>::U];  // the warp's first piece is on its way while rows are worked out
+  if (item < hi && item % P < p.pieces) load_piece(p, item / P, item % P, first);
+  auto count = [&](int i, int e) {
+    if (e >= 0) atomicAdd((i < i1 ? before : start) + e, 1);
     if (i >= i0 && i < i1) ids[i - i0] = e;
+  };
+  const int quads = p.vec_ids && n >= 4 * threads ? n >> 2 : 0;
+#pragma unroll 2
+  for (int q = tid; q < quads; q += threads) {
+    int e[4];
+    experts_of(a, q, e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) count(4 * q + j, e[j]);
   }
+  for (int i = 4 * quads + tid; i < n; i += threads) count(i, expert_of(a, i));
+  __syncthreads();
+  for (int e = tid; e < a.experts; e += threads) start[e] += before[e];
   __syncthreads();
   const int total = exclusive_scan(start, a.experts, warp_sums);
   // an entry's rank is the count up to the CTA's end less the own entries of its expert from it on
@@ -163,20 +222,24 @@ __global__ void __launch_bounds__(512) sort_tokens_kernel(const SortParams p) {
     const int j = j0 + lane;
     const int e = j < i1 - i0 ? ids[j] : -1;
     int from_here = __popc(__match_any_sync(0xffffffffu, e) & (0xffffffffu << lane));
-    for (int q = j0 + 32; q < i1 - i0; ++q) from_here += ids[q] == e;
-    if (j < i1 - i0) ids[i1 - i0 + j] = e < 0 ? -1 : start[e] + before[e] - from_here;
+#pragma unroll 4
+    for (int q = j0 + 32; q < i1 - i0; q += 4) {
+      const int4 later = *reinterpret_cast<const int4*>(ids + q);
+      from_here += (later.x == e) + (later.y == e) + (later.z == e) + (later.w == e);
+    }
+    if (j < i1 - i0) rows[j] = e < 0 ? -1 : start[e] + before[e] - from_here;
   }
   __syncthreads();
-  const int32_t* rows = ids + (i1 - i0);
   if (blockIdx.x == 0) {
     for (int e = tid; e < a.experts; e += threads) a.offsets[e] = start[e];
     if (tid == 0) a.offsets[a.experts] = total;
   }
-  for (int item = lo + (tid >> 5); item < hi; item += threads >> 5) {
+  for (bool ahead = true; item < hi; item += threads >> 5, ahead = false) {
     const int t = item / P, piece = item - t * P;
     const int row = lane < a.k ? rows[t * a.k - i0 + lane] : -1;
     if (piece == 0 && lane < a.k) a.row_of[t * a.k + lane] = row;
-    copy_piece<V>(p, t, piece, row);
+    if (!ahead && piece < p.pieces) load_piece(p, t, piece, first);
+    store_piece(p, t, piece, row, first);
   }
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, n, (int)blockIdx.x, (int)gridDim.x);
 }
@@ -185,7 +248,7 @@ __global__ void __launch_bounds__(512) sort_tokens_kernel(const SortParams p) {
 // of their own inside it, so that order needs no other means than a prefix over warps.
 // work: [chunk][expert] counts, then a rank for each entry.
 __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
-  extern __shared__ int32_t smem[];  // [warp][expert]
+  extern __shared__ __align__(16) int32_t smem[];  // [warp][expert]
   const SortTokensArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
   const int c = blockIdx.x;
@@ -198,19 +261,32 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
   const int w0 = min(i1, i0 + warp * each), w1 = min(i1, w0 + each);
   int32_t* own = smem + warp * a.experts;
   int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
-  for (int i = w0 + lane; i - lane < w1; i += 32) {
-    const int e = i < w1 ? expert_of(a, i) : -1;
+  auto rank_of = [&](int e) {  // among the warp's entries so far (every lane has one, or -1)
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     int rank = 0;
     if (e >= 0) rank = own[e] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
     if (e >= 0 && (same >> lane) == 1u) own[e] = rank + 1;  // (the last of them)
     __syncwarp();
+    return rank;
+  };
+  constexpr int kHeld = 4;  // entries that a lane keeps until the warps before it are known; beyond them it reads again
+  int held_id[kHeld], held_rank[kHeld];
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) {
+    const int i = w0 + 32 * r + lane;
+    held_id[r] = i < w1 ? expert_of(a, i) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) held_rank[r] = rank_of(held_id[r]);
+  for (int i = w0 + 32 * kHeld + lane; i - lane < w1; i += 32) {
+    const int rank = rank_of(i < w1 ? expert_of(a, i) : -1);
     if (i < w1) ranks[i] = rank;
   }
   __syncthreads();
   for (int e = tid; e < a.experts; e += blockDim.x) {
     int run = 0;
+#pragma unroll 8
     for (int w = 0; w < warps; ++w) {
       const int n = smem[w * a.experts + e];
       smem[w * a.experts + e] = run;
@@ -219,55 +295,73 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
     a.work[(int64_t)c * a.experts + e] = run;
   }
   __syncthreads();
-  for (int i = w0 + lane; i < w1; i += 32) {
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) {
+    const int i = w0 + 32 * r + lane;
+    if (i < w1) ranks[i] = held_id[r] >= 0 ? held_rank[r] + own[held_id[r]] : 0;
+  }
+  for (int i = w0 + 32 * kHeld + lane; i < w1; i += 32) {
     const int e = expert_of(a, i);
     if (e >= 0) ranks[i] += own[e];
   }
 }
 
-// The second: a CTA adds up the runs' counts, and copies its share of one run's rows.
+// The second: a CTA adds up the runs' counts, and copies its share of the rows, which lies in one run or two.
 template <typename V>
-__global__ void __launch_bounds__(512) sort_scatter_kernel(const SortParams p) {
-  extern __shared__ int32_t smem[];
+__global__ void __launch_bounds__(512, 3) sort_scatter_kernel(const SortParams p) {
+  extern __shared__ __align__(16) int32_t smem[];
   __shared__ int32_t warp_sums[32];
   const SortTokensArgs& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x, warps = threads >> 5;
-  const int c = (int)blockIdx.x / p.ctas_of_chunk, g = (int)blockIdx.x - c * p.ctas_of_chunk;
-  int32_t* start = smem;
-  int32_t* base = start + a.experts;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warps = threads >> 5;
+  const int P = p.pieces + (a.scale != nullptr);
+  const int64_t items = (int64_t)a.tokens * P;
+  const int64_t lo = items * blockIdx.x / gridDim.x, hi = items * (blockIdx.x + 1) / gridDim.x;
+  const int run = (int)(lo / P) / p.chunk_tokens, t_next = (run + 1) * p.chunk_tokens;
+  int32_t* start = smem;              // all entries of an expert, then its first row
+  int32_t* base = start + a.experts;  // first row of the share's first run, and of the next
+  int32_t* next = base + a.experts;
+  for (int e = tid; e < 2 * a.experts; e += threads) smem[e] = 0;
+  __syncthreads();
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  for (int e = tid; e < a.experts; e += threads) {
+  const int slices = max(1, threads / a.experts);  // of the runs, which threads of the same expert share
+  for (int i = tid; i < slices * a.experts; i += threads) {
+    const int e = i % a.experts;
     int all = 0, earlier = 0;
-    for (int q = 0; q < p.chunks; ++q) {
+#pragma unroll 8
+    for (int q = i / a.experts; q < p.chunks; q += slices) {
       const int n = __ldcg(a.work + (int64_t)q * a.experts + e);
       all += n;
-      earlier += q < c ? n : 0;
+      earlier += q < run ? n : 0;
+      if (q == run) next[e] = n;
     }
-    start[e] = all;
-    base[e] = earlier;
+    atomicAdd(start + e, all);
+    atomicAdd(base + e, earlier);
   }
   __syncthreads();
   const int total = exclusive_scan(start, a.experts, warp_sums);
+  for (int e = tid; e < a.experts; e += threads) {
+    base[e] += start[e];
+    next[e] += base[e];
+  }
   if (blockIdx.x == 0) {
     for (int e = tid; e < a.experts; e += threads) a.offsets[e] = start[e];
     if (tid == 0) a.offsets[a.experts] = total;
   }
-  const int P = p.pieces + (a.scale != nullptr);
-  const int t0 = c * p.chunk_tokens, t1 = min(a.tokens, t0 + p.chunk_tokens);
-  const int64_t items = (int64_t)(t1 - t0) * P;
-  const int64_t lo = items * g / p.ctas_of_chunk, hi = items * (g + 1) / p.ctas_of_chunk;
+  __syncthreads();
   const int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
   for (int64_t item = lo + (tid >> 5); item < hi; item += warps) {
-    const int t = t0 + (int)(item / P), piece = (int)(item % P);
+    const int t = (int)(item / P), piece = (int)(item - (int64_t)t * P);
+    V r[Copy<V>::U];
+    if (piece < p.pieces) load_piece(p, t, piece, r);
     int row = -1;
     if (lane < a.k) {
       const int64_t i = (int64_t)t * a.k + lane;
       const int e = expert_of(a, i);
-      if (e >= 0) row = start[e] + base[e] + __ldcg(ranks + i);
+      if (e >= 0) row = (t < t_next ? base : next)[e] + __ldcg(ranks + i);
       if (piece == 0) a.row_of[i] = row;
     }
-    copy_piece<V>(p, t, piece, row);
+    store_piece(p, t, piece, row, r);
   }
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, (int64_t)a.tokens * a.k, (int)blockIdx.x, (int)gridDim.x);
 }
@@ -303,9 +397,9 @@ struct UnsortBackwardParams {
 
 }  // namespace
 
-// A warp takes a piece of a token's row: U vectors a lane of KB rows at a time.
-template <typename T, bool VEC, int KB>
-__global__ void __launch_bounds__(256) unsort_tokens_kernel(const UnsortParams p) {
+// A warp takes a piece of a token's row: U vectors a lane of KB rows at a time.  CTAS of a kernel fit an SM.
+template <typename T, bool VEC, int KB, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) unsort_tokens_kernel(const UnsortParams p) {
   using B = Bit<T, VEC>;
   using Raw = typename B::Raw;
   constexpr int U = VEC ? 2 : 4;
@@ -362,11 +456,11 @@ __global__ void __launch_bounds__(256) unsort_tokens_kernel(const UnsortParams p
 
 // A CTA takes a token.  DOT: the weights' gradient is wanted, so the rows are read.
 template <typename T, bool VEC, bool DOT>
-__global__ void __launch_bounds__(256) unsort_tokens_backward_kernel(const UnsortBackwardParams p) {
+__global__ void __launch_bounds__(1024) unsort_tokens_backward_kernel(const UnsortBackwardParams p) {
   using B = Bit<T, VEC>;
   using Raw = typename B::Raw;
   constexpr int KB = 4;
-  __shared__ float parts[8][kSortMaxTopk];
+  __shared__ float parts[32][kSortMaxTopk];
   const UnsortBackwardArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
   const int64_t row_bytes = (int64_t)a.hidden * (int64_t)sizeof(T);
@@ -454,12 +548,15 @@ __global__ void __launch_bounds__(256) unsort_tokens_backward_kernel(const Unsor
 // ---------------------------------------------------------------------------------------
 namespace {
 
-constexpr int64_t kOneLaunchEntries = 16384;
-constexpr int kMaxChunks = 64;
+constexpr int64_t kOneLaunchEntries = 32768;
+constexpr int kMaxChunks = 256;
+// Shared memory that keeps a CTA alone on its SM: where two fit, a launch that starts while the one before it still runs may
+// put two on the SMs that happen to be free, and none on others.
+constexpr int kAloneBytes = 116 * 1024;
 constexpr int kCountSmem = 160 * 1024;  // of the counting kernel: a count of every expert for each warp
 
 int sort_chunks(int64_t tokens, int k) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxChunks, tokens * k / 2048));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxChunks, tokens * k / 4096));
 }
 
 template <typename V>
@@ -471,16 +568,22 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
   const int64_t items = (int64_t)a.tokens * (p.pieces + (a.scale != nullptr));
   if (a.work == nullptr) {
     if (items > INT32_MAX) return cudaErrorInvalidValue;
-    const int threads = 512;
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + 15) / 16, 2 * (int64_t)sms));
+    // Every CTA counts all entries: few large ones repeat less of that where there are many.  Up to 16 pieces an SM, one to
+    // a warp and one CTA to an SM.
+    const int64_t share = (items + sms - 1) / sms;
+    const bool few = share <= 16;
+    const int threads = few ? 32 * (int)std::max<int64_t>(4, share) : (int64_t)a.tokens * a.k > 2048 ? 1024 : 512;
+    const int warps = threads / 32;
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + warps - 1) / warps, (few ? 1 : 1024 / threads) * (int64_t)sms));
     const int P = p.pieces + (a.scale != nullptr);
     const int64_t own = ((items + grid - 1) / grid + 2 * P - 2) / P * a.k;  // entries of the tokens that a CTA touches, at most
-    const size_t smem = (2 * (size_t)a.experts + 2 * (size_t)own) * sizeof(int32_t);
+    const size_t smem = 2 * ((size_t)((a.experts + 3) & ~3) + (size_t)((own + 3) & ~3)) * sizeof(int32_t);
     static OncePerDevice once;
     const cudaError_t opted = once([] { return opt_in(sort_tokens_kernel<V>, kCountSmem, false); });
     if (opted != cudaSuccess) return opted;
     if (smem > kCountSmem) return cudaErrorInvalidValue;
-    return ptx::launch_dependent(sort_tokens_kernel<V>, grid, threads, smem, stream, p);
+    const size_t alone = few ? std::max<size_t>(smem, kAloneBytes) : smem;
+    return ptx::launch_dependent(sort_tokens_kernel<V>, grid, threads, alone, stream, p);
   }
   p.chunks = sort_chunks(a.tokens, a.k);
   p.chunk_tokens = (a.tokens + p.chunks - 1) / p.chunks;
@@ -488,16 +591,16 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
   static OncePerDevice once;
   const cudaError_t opted = once([] {
     const cudaError_t e = opt_in(sort_count_kernel, kCountSmem, false);
-    return e != cudaSuccess ? e : opt_in(sort_scatter_kernel<V>, 2 * kSortMaxExperts * (int)sizeof(int32_t), false);
+    return e != cudaSuccess ? e : opt_in(sort_scatter_kernel<V>, 3 * kSortMaxExperts * (int)sizeof(int32_t), false);
   });
   if (opted != cudaSuccess) return opted;
   const int warps = std::max(1, std::min(32, kCountSmem / (a.experts * (int)sizeof(int32_t))));
   cudaError_t e = ptx::launch_dependent(sort_count_kernel, p.chunks, 32 * warps, (size_t)warps * a.experts * sizeof(int32_t),
                                         stream, p);
   if (e != cudaSuccess) return e;
-  p.ctas_of_chunk = std::max(1, (2 * sms + p.chunks - 1) / p.chunks);
-  return ptx::launch_dependent(sort_scatter_kernel<V>, p.chunks * p.ctas_of_chunk, 512, 2 * (size_t)a.experts * sizeof(int32_t),
-                               stream, p);
+  // (a share is no longer than a run: there are more CTAs than runs)
+  const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>((items + 15) / 16, 3 * (int64_t)sms));
+  return ptx::launch_dependent(sort_scatter_kernel<V>, grid, 512, 3 * (size_t)a.experts * sizeof(int32_t), stream, p);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -509,13 +612,17 @@ cudaError_t unsort_typed(const UnsortTokensArgs& a, int sms, cudaStream_t stream
   p.row_vecs = a.hidden / Bit<T, VEC>::N;
   p.piece_vecs = VEC ? 64 : 128;
   p.pieces = (p.row_vecs + p.piece_vecs - 1) / p.piece_vecs;
-  const int64_t items = (int64_t)a.tokens * p.pieces;
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, 4 * (int64_t)sms));
-  switch (a.k) {
-    case 1: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 1>, grid, 256, 0, stream, p);
-    case 2: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 2>, grid, 256, 0, stream, p);
-    default: return ptx::launch_dependent(unsort_tokens_kernel<T, VEC, 4>, grid, 256, 0, stream, p);
-  }
+  // Many pieces: four CTAs to an SM, and twice as many in the grid, which evens out what some lose on memory (bf16, us: 4096
+  // tokens, top-6, rows of 8 KiB 50 with as many as would fit with more registers, 39; 2047, top-8 28.8, 25.9; 2047, top-4,
+  // 5760 bytes 12.2, 10.8).  Few: every row of a token at once (128 tokens, top-8, 14 KiB 5.4, 4.3).
+  const int64_t ctas = ((int64_t)a.tokens * p.pieces + 7) / 8;
+  const bool few = ctas <= 2 * (int64_t)sms;
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(ctas, 8 * (int64_t)sms));
+  const auto go = [&](auto kernel) { return ptx::launch_dependent(kernel, grid, 256, 0, stream, p); };
+  if (a.k == 1) return go(unsort_tokens_kernel<T, VEC, 1, 4>);
+  if (a.k == 2) return go(unsort_tokens_kernel<T, VEC, 2, 4>);
+  if (few) return a.k <= 4 ? go(unsort_tokens_kernel<T, VEC, 4, 2>) : go(unsort_tokens_kernel<T, VEC, 8, 2>);
+  return go(unsort_tokens_kernel<T, VEC, 4, 4>);
 }
 
 template <typename T>
@@ -529,7 +636,10 @@ cudaError_t backward_typed(const UnsortBackwardArgs& a, int sms, cudaStream_t st
   UnsortBackwardParams p;
   p.a = a;
   p.row_vecs = a.hidden / Bit<T, VEC>::N;
-  const int threads = std::max(32, std::min(256, (p.row_vecs / 2 + 31) / 32 * 32));
+  // Two vectors a lane, or one where there are few tokens, and then up to 1024 lanes (us: 128 tokens, top-8, 14 KiB 9.7 with two
+  // and 256 lanes, 6.1; 256 of them 15.0, with one and 512 lanes 10.4; 4096, top-6, 8 KiB 75.9 with two, 86.5 with one).
+  const int each = a.tokens <= 4 * sms ? 1 : 2;
+  const int threads = std::max(32, std::min(a.tokens <= sms ? 1024 : 512, (p.row_vecs / each + 31) / 32 * 32));
   const int grid = (int)std::min<int64_t>(std::max(a.tokens, 1), 1 << 30);
   return a.grad_weights != nullptr
              ? ptx::launch_dependent(unsort_tokens_backward_kernel<T, VEC, true>, grid, threads, 0, stream, p)
@@ -556,8 +666,10 @@ cudaError_t launch_sort_tokens(const SortTokensArgs& a, int sms, cudaStream_t st
     return cudaErrorInvalidValue;
   SortParams p = {};
   p.a = a;
+  p.vec_ids = (reinterpret_cast<uintptr_t>(a.indices) & 15u) == 0;
   const uint64_t bits = (uint64_t)a.row_bytes | (uint64_t)a.x_stride | reinterpret_cast<uintptr_t>(a.x) |
                         reinterpret_cast<uintptr_t>(a.rows);
+  if (bits % 32 == 0) return sort_typed<Vec32>(p, sms, stream);
   if (bits % 16 == 0) return sort_typed<int4>(p, sms, stream);
   if (bits % 4 == 0) return sort_typed<int>(p, sms, stream);
   if (bits % 2 == 0) return sort_typed<short>(p, sms, stream);

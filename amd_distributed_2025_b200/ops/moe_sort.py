@@ -28,6 +28,9 @@ from torch.autograd.function import once_differentiable
 from . import _ext
 
 
+_tuple = tuple.__new__  # (what the classes below do in Python on every call takes as long as a short kernel's launch)
+
+
 class ExpertOrder(NamedTuple):
     """Where the rows of the entries lie."""
 
@@ -51,14 +54,15 @@ def sort_tokens(
 
     ``scale [T, S]`` (fp32) goes the same way: the block scales of e4m3 rows."""
     ext = _ext.load()
-    if x.requires_grad and torch.is_grad_enabled():
-        if scale is not None:
-            raise ValueError("rows with scales have no gradient: call sort_tokens under torch.no_grad()")
+    got = ext.sort_tokens(x, indices, num_experts, scale)
+    if got is None:  # x wants a gradient
+        if scale is not None or x.element_size() == 1:
+            raise ValueError("e4m3 rows and rows with scales have no gradient: call sort_tokens under torch.no_grad()")
         _refuse_foreign_leaves(ext, x)
         rows, offsets, row_of = _Sort.apply(x, indices, num_experts)
         return SortedTokens(rows, None, ExpertOrder(offsets, row_of))
-    rows, rows_scale, offsets, row_of = ext.sort_tokens(x, indices, num_experts, scale)
-    return SortedTokens(rows, rows_scale, ExpertOrder(offsets, row_of))
+    rows, rows_scale, offsets, row_of = got
+    return _tuple(SortedTokens, (rows, rows_scale, _tuple(ExpertOrder, (offsets, row_of))))
 
 
 def unsort_tokens(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -66,18 +70,21 @@ def unsort_tokens(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torc
 
     ``rows [T k, H]`` in fp16, bf16 or fp32; ``weights [T, k]`` in a floating type."""
     ext = _ext.load()
+    out = ext.unsort_tokens(rows, order.row_of, weights)
+    if out is not None:
+        return out
     if weights is not None and weights.dtype != torch.float32:
+        if not weights.dtype.is_floating_point:
+            raise ValueError(f"weights must be of a floating type, not {weights.dtype}")
         weights = weights.to(torch.float32)
-    wants = rows.requires_grad or (weights is not None and weights.requires_grad)
-    if wants and torch.is_grad_enabled():
-        _refuse_foreign_leaves(ext, rows, weights)
-        return _Unsort.apply(rows, order.offsets, order.row_of, weights)
-    return ext.unsort_tokens(rows, order.row_of, weights)
+    _refuse_foreign_leaves(ext, rows, weights)
+    return _Unsort.apply(rows, order.offsets, order.row_of, weights)
 
 
 def sort_tokens_backward(grad_rows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """Gradient of ``x`` from that of ``sort_tokens(x, ...).rows``: each token's rows added up."""
-    return _ext.load().unsort_tokens(grad_rows, order.row_of, None)
+    with torch.no_grad():
+        return _ext.load().unsort_tokens(grad_rows, order.row_of, None)
 
 
 def unsort_tokens_backward(
@@ -85,7 +92,7 @@ def unsort_tokens_backward(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of ``rows`` and of ``weights`` (fp32; None without weights) from that of ``unsort_tokens(...)``."""
     if weights is not None and weights.dtype != torch.float32:
-        weights = weights.to(torch.float32)
+        weights = weights.detach().to(torch.float32)
     return _ext.load().unsort_tokens_backward(grad, rows, order.offsets, order.row_of, weights, True, True)
 
 

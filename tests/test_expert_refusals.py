@@ -70,6 +70,7 @@ def test_sort_tokens_refusals():
     _refused("scale must be", lambda: f(x, ids, 8, scale=F(3, 1)))
     _refused("scale must be", lambda: f(x, ids, 8, scale=F(4, 1).half()))
     _refused("no gradient", lambda: f(x.clone().requires_grad_(), ids, 8, scale=F(4, 1)))
+    _refused("no gradient", lambda: f(x.to(torch.float8_e4m3fn).requires_grad_(), ids, 8))
     _refused("CUDA", lambda: f(x, ids, 8))
 
 
@@ -83,6 +84,7 @@ def test_unsort_tokens_refusals():
     _refused("a row for each", lambda: f(F(9, 64), order, w))
     _refused("weights must be", lambda: f(rows, order, F(4, 3)))
     _refused("weights must be", lambda: f(rows, order, F(8)))
+    _refused("floating type", lambda: f(rows, order, F(4, 2, dtype=torch.int32)))
     _refused("row_of must be", lambda: f(rows, ExpertOrder(order.offsets, order.row_of.long()), w))
     _refused("row_of must be", lambda: f(rows, ExpertOrder(order.offsets, order.row_of[0]), w))
     _refused("CUDA", lambda: f(rows, order, w))

@@ -637,6 +637,14 @@ def test_fp8_grouped_gemm(counts, n, k):
     assert f.fp8_grouped_gemm(*inputs, c=given) is given and torch.equal(given, out)
 
 
+def test_fp8_grouped_gemm_keeps_its_sums_in_registers():
+    from amd_distributed_2025_b200.ops import _ext
+
+    ext = _ext.load()
+    assert [ext.fp8_grouped_local_bytes(tile) for tile in (64, 256)] == [0, 0]
+    assert ext.fp8_grouped_tile(72 * 8 + 7, 8) == 64 and ext.fp8_grouped_tile(73 * 8, 8) == 256
+
+
 def test_fp8_grouped_gemm_matches_fp8_gemm():
     """One expert is fp8_gemm (the same sums in the same order, but the two scales are multiplied first in both)."""
     from amd_distributed_2025_b200.ops.fp8_gemm import fp8_gemm, fp8_grouped_gemm
