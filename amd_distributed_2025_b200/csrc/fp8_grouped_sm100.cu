@@ -99,13 +99,27 @@ struct Tables {
   int32_t *start, *count, *tiles_end;
 };
 
+// A pair's tiles: dealt out in turn, every other round the other way round.  Were it always the same, the token tiles of
+// experts with 384 rows each, 256 and 128, would go to even and to odd pairs for good (64 of them: 533 us, 412).  (A tile from
+// the front of the list and one from its end in turn, or a run of it to each pair, evens out as much and takes L2 its sense:
+// skewed routing 493 and 645 us against 480.)
 template <int BT>
 struct Walk {
-  const Tables& t;
-  int n_tiles;
-  int e = 0;
-  __device__ __forceinline__ Tile at(int tile) {
-    while (tile >= t.tiles_end[e]) ++e;
+  Tables t;
+  int experts;
+  // The pair's tile of a round, or -1 behind the last.
+  __device__ __forceinline__ int tile_of(int round) const {
+    const int pairs = (int)gridDim.x >> 1, pair = (int)blockIdx.x >> 1;
+    const int tile = round * pairs + ((round & 1) != 0 ? pairs - 1 - pair : pair);
+    return tile < t.tiles_end[experts - 1] ? tile : -1;
+  }
+  __device__ __forceinline__ Tile at(int tile) const {
+    int e = 0;
+    for (int above = experts; above - e > 0;) {  // the first whose tiles end behind this one
+      const int m = (e + above) >> 1;
+      if (t.tiles_end[m] > tile) above = m;
+      else e = m + 1;
+    }
     const int local = tile - (e > 0 ? t.tiles_end[e - 1] : 0);
     const int count = t.count[e];
     const int parts = (count + BT - 1) / BT;
@@ -215,9 +229,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   ptx::cluster_sync_all();
   ptx::tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_shared;
-  const int total = tables.tiles_end[p.experts - 1];
-  const int first_tile = (int)blockIdx.x >> 1, tile_step = (int)gridDim.x >> 1;
-  Walk<kBt> walk{tables, p.n_tiles};
+  const Walk<kBt> walk{tables, p.experts};
   // K blocks that are multiplied into a tensor-memory buffer one beside the other.
   auto steps = [](int width) { return WIDE ? 2 * kRows / width : 4; };
 
@@ -241,7 +253,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     ptx::setmaxnreg_dec<kLightRegs>();
     if (warp == 0) {
       uint32_t stage = 0, phase = 0;
-      for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
+      for (int round = 0, tile; (tile = walk.tile_of(round)) >= 0 && !abort_flag; ++round) {
         const Tile t = walk.at(tile);
         const int by = t.expert * p.N + t.nt * 2 * kRows + cta * kRows;
         const int half = t.width / 2;  // tokens that this CTA brings in
@@ -268,7 +280,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     } else if (warp == 1) {
       if (cta == 0) {
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-        for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
+        for (int round = 0, tile; (tile = walk.tile_of(round)) >= 0 && !abort_flag; ++round) {
           const Tile t = walk.at(tile);
           const uint32_t idesc = WIDE ? make_idesc_e4m3_f32(t.width, 2 * kRows) : make_idesc_e4m3_f32(2 * kRows, t.width);
           const int step = steps(t.width);
@@ -313,7 +325,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       // epilogue's lanes read them.
       const int l = (warp - 2) * 32 + lane;
       uint32_t slot = 0, phase = 0;
-      for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
+      for (int round = 0, tile; (tile = walk.tile_of(round)) >= 0 && !abort_flag; ++round) {
         const Tile t = walk.at(tile);
         const int last = (p.N - 1) >> 7;
         const float* bs = p.b_scale + t.expert * p.bs_stride_e;
@@ -435,7 +447,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       }
       __syncwarp();
     };
-    for (int tile = first_tile; tile < total && !abort_flag; tile += tile_step) {
+    for (int round = 0, tile; (tile = walk.tile_of(round)) >= 0 && !abort_flag; ++round) {
       const Tile t = walk.at(tile);
       if (WIDE && t.width == 2 * kRows) {
         // ---- tokens in lanes: a lane's scale is its token's times that of its columns' block of weights -------
