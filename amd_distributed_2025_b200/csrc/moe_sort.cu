@@ -56,7 +56,7 @@ __device__ __forceinline__ void store_vec<Vec32>(Vec32* p, const Vec32& v) {
 
 struct SortParams {
   SortTokensArgs a;
-  int32_t pieces;      // of a row; the scales are one more
+  int32_t pieces;      // of a row
   int32_t row_vecs, piece_vecs;
   int32_t vec_ids;               // 1: ids begin at a multiple of 16 bytes
   int32_t chunks, chunk_tokens;  // two launches: runs of tokens that are counted by a CTA each
@@ -112,50 +112,51 @@ __device__ __forceinline__ int exclusive_scan(int32_t* counts, int n, int32_t* w
   return total;
 }
 
-// One piece of token t's row: a warp asks for it ...
+// One piece of token t's row, and with the first one its scales (two a lane; more are read when they are stored).  Warps ask
+// for the next piece before they store the one at hand: a load that is issued behind stores waits for them.
 template <typename V>
-__device__ __forceinline__ void load_piece(const SortParams& p, int t, int piece, V* r) {
-  constexpr int U = Copy<V>::U;
+struct Piece {
+  V r[Copy<V>::U];
+  float s[2];
+};
+template <typename V>
+__device__ __forceinline__ void load_piece(const SortParams& p, int t, int piece, Piece<V>& to) {
+  const int lane = threadIdx.x & 31;
   const V* src = reinterpret_cast<const V*>(reinterpret_cast<const uint8_t*>(p.a.x) + (int64_t)t * p.a.x_stride);
-  const int v0 = piece * p.piece_vecs + (int)(threadIdx.x & 31);
+  const int v0 = piece * p.piece_vecs + lane;
   const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (v0 + 32 * u < v1) r[u] = load_vec(src + v0 + 32 * u);
+  for (int u = 0; u < Copy<V>::U; ++u)
+    if (v0 + 32 * u < v1) to.r[u] = load_vec(src + v0 + 32 * u);
+  if (piece == 0 && p.a.scale != nullptr) {
+    const float* scale = p.a.scale + (int64_t)t * p.a.scale_stride;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 32 * u < p.a.scale_cols) to.s[u] = __ldcg(scale + lane + 32 * u);
+  }
 }
-// ... and stores it to the token's k rows; `row` is lane j's: entry j's row.  (Behind the last piece: the token's scales.)
+// Stores it to the token's k rows; `row` is lane j's: entry j's row.
 template <typename V>
-__device__ __forceinline__ void store_piece(const SortParams& p, int t, int piece, int row, const V* r) {
-  constexpr int U = Copy<V>::U;
+__device__ __forceinline__ void store_piece(const SortParams& p, int t, int piece, int row, const Piece<V>& from) {
   const int lane = threadIdx.x & 31;
   const SortTokensArgs& a = p.a;
-  if (piece < p.pieces) {
-    const int v0 = piece * p.piece_vecs + lane;
-    const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
-    for (int j = 0; j < a.k; ++j) {
-      const int to = __shfl_sync(0xffffffffu, row, j);
-      if (to < 0) continue;
-      V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(a.rows) + (int64_t)to * a.row_bytes);
+  const int v0 = piece * p.piece_vecs + lane;
+  const int v1 = min(p.row_vecs, (piece + 1) * p.piece_vecs);
+  const bool scales = piece == 0 && a.scale != nullptr;
+  if (piece == 0 && lane < a.k) a.row_of[(int64_t)t * a.k + lane] = row;
+  for (int j = 0; j < a.k; ++j) {
+    const int to = __shfl_sync(0xffffffffu, row, j);
+    if (to < 0) continue;
+    V* dst = reinterpret_cast<V*>(reinterpret_cast<uint8_t*>(a.rows) + (int64_t)to * a.row_bytes);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v0 + 32 * u < v1) store_vec(dst + v0 + 32 * u, r[u]);
-    }
-  } else {
-    // A row's scales are no whole number of cache lines, and its neighbours' come at another time: lines that are written in
-    // parts stay in L2 until they are complete (65536 rows of 224 bytes: 126 us -> SCALEUS).
-    uint64_t policy;
-    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
-    const float* src = a.scale + (int64_t)t * a.scale_stride;
-    for (int c0 = 0; c0 < a.scale_cols; c0 += 32) {
-      const bool in = c0 + lane < a.scale_cols;
-      const float s = in ? __ldcg(src + c0 + lane) : 0.f;
-      for (int j = 0; j < a.k; ++j) {
-        const int to = __shfl_sync(0xffffffffu, row, j);
-        if (to >= 0 && in)
-          asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(a.rows_scale + (int64_t)to * a.scale_cols + c0 + lane),
-                       "f"(s), "l"(policy)
-                       : "memory");
-      }
+    for (int u = 0; u < Copy<V>::U; ++u)
+      if (v0 + 32 * u < v1) store_vec(dst + v0 + 32 * u, from.r[u]);
+    if (scales) {
+      float* scale = a.rows_scale + (int64_t)to * a.scale_cols;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane + 32 * u < a.scale_cols) scale[lane + 32 * u] = from.s[u];
+      for (int c = lane + 64; c < a.scale_cols; c += 32) scale[c] = __ldcg(a.scale + (int64_t)t * a.scale_stride + c);
     }
   }
 }
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(const SortParams p) {
   __shared__ int32_t warp_sums[32];
   const SortTokensArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x;
-  const int P = p.pieces + (a.scale != nullptr);
+  const int P = p.pieces;
   const int64_t items = (int64_t)a.tokens * P;
   const int lo = (int)(items * blockIdx.x / gridDim.x), hi = (int)(items * (blockIdx.x + 1) / gridDim.x);
   const int t0 = lo / P, t1 = hi > lo ? (hi + P - 1) / P : t0;
@@ -198,8 +199,8 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(const SortParams p) {
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   int item = lo + (tid >> 5);
-  V first[Copy<V>::U];  // the warp's first piece is on its way while rows are worked out
-  if (item < hi && item % P < p.pieces) load_piece(p, item / P, item % P, first);
+  Piece<V> next;  // the warp's first piece is on its way while rows are worked out
+  if (item < hi) load_piece(p, item / P, item % P, next);
   auto count = [&](int i, int e) {
     if (e >= 0) atomicAdd((i < i1 ? before : start) + e, 1);
     if (i >= i0 && i < i1) ids[i - i0] = e;
@@ -234,12 +235,11 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(const SortParams p) {
     for (int e = tid; e < a.experts; e += threads) a.offsets[e] = start[e];
     if (tid == 0) a.offsets[a.experts] = total;
   }
-  for (bool ahead = true; item < hi; item += threads >> 5, ahead = false) {
-    const int t = item / P, piece = item - t * P;
-    const int row = lane < a.k ? rows[t * a.k - i0 + lane] : -1;
-    if (piece == 0 && lane < a.k) a.row_of[t * a.k + lane] = row;
-    if (!ahead && piece < p.pieces) load_piece(p, t, piece, first);
-    store_piece(p, t, piece, row, first);
+  for (const int warps = threads >> 5; item < hi; item += warps) {
+    const Piece<V> now = next;
+    if (item + warps < hi) load_piece(p, (item + warps) / P, (item + warps) % P, next);
+    const int t = item / P;
+    store_piece(p, t, item - t * P, lane < a.k ? rows[t * a.k - i0 + lane] : -1, now);
   }
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, n, (int)blockIdx.x, (int)gridDim.x);
 }
@@ -307,13 +307,19 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
 }
 
 // The second: a CTA adds up the runs' counts, and copies its share of the rows, which lies in one run or two.
+//
+// Bound by the row stores, which memory takes the slower the more of them are under way in different places: 65536 rows of
+// 7168 bytes with scales (8192 tokens, top-8) take 118 us with 16 to 32 warps an SM, 123 to 126 with 48, 134 with 64; as bare
+// copies, without the counting and the scales, 93 to 100.  (Scales as a piece of their own, whose loads wait behind the stores
+// of others: 126 with 32 warps.  In the order of the rows instead of the tokens': 115 and more for the copies alone.)
+constexpr int kScatterThreads = 512, kScatterCtas = 2;
 template <typename V>
-__global__ void __launch_bounds__(512, 3) sort_scatter_kernel(const SortParams p) {
+__global__ void __launch_bounds__(kScatterThreads, kScatterCtas) sort_scatter_kernel(const SortParams p) {
   extern __shared__ __align__(16) int32_t smem[];
   __shared__ int32_t warp_sums[32];
   const SortTokensArgs& a = p.a;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warps = threads >> 5;
-  const int P = p.pieces + (a.scale != nullptr);
+  const int P = p.pieces;
   const int64_t items = (int64_t)a.tokens * P;
   const int64_t lo = items * blockIdx.x / gridDim.x, hi = items * (blockIdx.x + 1) / gridDim.x;
   const int run = (int)(lo / P) / p.chunk_tokens, t_next = (run + 1) * p.chunk_tokens;
@@ -350,18 +356,24 @@ __global__ void __launch_bounds__(512, 3) sort_scatter_kernel(const SortParams p
   }
   __syncthreads();
   const int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
-  for (int64_t item = lo + (tid >> 5); item < hi; item += warps) {
-    const int t = (int)(item / P), piece = (int)(item - (int64_t)t * P);
-    V r[Copy<V>::U];
-    if (piece < p.pieces) load_piece(p, t, piece, r);
-    int row = -1;
+  int64_t item = lo + (tid >> 5);
+  Piece<V> next_piece;
+  int next_id = -1, next_rank = 0;
+  auto ask = [&](int64_t i) {
+    const int t = (int)(i / P);
+    load_piece(p, t, (int)(i - (int64_t)t * P), next_piece);
     if (lane < a.k) {
-      const int64_t i = (int64_t)t * a.k + lane;
-      const int e = expert_of(a, i);
-      if (e >= 0) row = (t < t_next ? base : next)[e] + __ldcg(ranks + i);
-      if (piece == 0) a.row_of[i] = row;
+      next_id = expert_of(a, (int64_t)t * a.k + lane);
+      next_rank = __ldcg(ranks + (int64_t)t * a.k + lane);
     }
-    store_piece(p, t, piece, row, r);
+  };
+  if (item < hi) ask(item);
+  for (; item < hi; item += warps) {
+    const Piece<V> now = next_piece;
+    const int t = (int)(item / P);
+    const int row = next_id >= 0 ? (t < t_next ? base : next)[next_id] + next_rank : -1;
+    if (item + warps < hi) ask(item + warps);
+    store_piece(p, t, (int)(item - (int64_t)t * P), row, now);
   }
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, (int64_t)a.tokens * a.k, (int)blockIdx.x, (int)gridDim.x);
 }
@@ -565,7 +577,7 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
   p.row_vecs = (int)(a.row_bytes / (int64_t)sizeof(V));
   p.piece_vecs = 32 * Copy<V>::U;
   p.pieces = std::max(1, (p.row_vecs + p.piece_vecs - 1) / p.piece_vecs);
-  const int64_t items = (int64_t)a.tokens * (p.pieces + (a.scale != nullptr));
+  const int64_t items = (int64_t)a.tokens * p.pieces;
   if (a.work == nullptr) {
     if (items > INT32_MAX) return cudaErrorInvalidValue;
     // Every CTA counts all entries: few large ones repeat less of that where there are many.  Up to 16 pieces an SM, one to
@@ -575,7 +587,7 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
     const int threads = few ? 32 * (int)std::max<int64_t>(4, share) : (int64_t)a.tokens * a.k > 2048 ? 1024 : 512;
     const int warps = threads / 32;
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((items + warps - 1) / warps, (few ? 1 : 1024 / threads) * (int64_t)sms));
-    const int P = p.pieces + (a.scale != nullptr);
+    const int P = p.pieces;
     const int64_t own = ((items + grid - 1) / grid + 2 * P - 2) / P * a.k;  // entries of the tokens that a CTA touches, at most
     const size_t smem = 2 * ((size_t)((a.experts + 3) & ~3) + (size_t)((own + 3) & ~3)) * sizeof(int32_t);
     static OncePerDevice once;
@@ -599,8 +611,9 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
                                         stream, p);
   if (e != cudaSuccess) return e;
   // (a share is no longer than a run: there are more CTAs than runs)
-  const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>((items + 15) / 16, 3 * (int64_t)sms));
-  return ptx::launch_dependent(sort_scatter_kernel<V>, grid, 512, 3 * (size_t)a.experts * sizeof(int32_t), stream, p);
+  const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>((items + kScatterThreads / 32 - 1) / (kScatterThreads / 32),
+                                                                     kScatterCtas * (int64_t)sms));
+  return ptx::launch_dependent(sort_scatter_kernel<V>, grid, kScatterThreads, 3 * (size_t)a.experts * sizeof(int32_t), stream, p);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

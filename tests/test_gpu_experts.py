@@ -296,7 +296,8 @@ def test_sort_tokens(tokens, k, experts, hidden, dtype, kind):
         _check_sort(x, ids, experts, sort_tokens(x, ids, experts))
 
 
-@pytest.mark.parametrize("tokens,k,experts,hidden", [(1, 8, 64, 7168), (101, 4, 128, 2880), (4096, 8, 64, 1111), (3, 2, 8, 130)])
+@pytest.mark.parametrize("tokens,k,experts,hidden", [(1, 8, 64, 7168), (101, 4, 128, 2880), (4096, 8, 64, 1111), (3, 2, 8, 130),
+                                                         (70, 3, 8, 12800), (5000, 8, 64, 8512)])
 def test_sort_tokens_e4m3_rows_with_scales(tokens, k, experts, hidden):
     from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
 
