@@ -309,9 +309,9 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
 // The second: a CTA adds up the runs' counts, and copies its share of the rows, which lies in one run or two.
 //
 // Bound by the row stores, which memory takes the slower the more of them are under way in different places: 65536 rows of
-// 7168 bytes with scales (8192 tokens, top-8) take 118 us with 16 to 32 warps an SM, 123 to 126 with 48, 134 with 64; as bare
+// 7168 bytes with scales (8192 tokens, top-8) take 111 us with 16 to 32 warps an SM, 5 to 8 more with 48, 16 more with 64; as bare
 // copies, without the counting and the scales, 93 to 100.  (Scales as a piece of their own, whose loads wait behind the stores
-// of others: 126 with 32 warps.  In the order of the rows instead of the tokens': 115 and more for the copies alone.)
+// of others: 8 us more.  In the order of the rows instead of the tokens': 115 and more for the copies alone.)
 constexpr int kScatterThreads = 512, kScatterCtas = 2;
 template <typename V>
 __global__ void __launch_bounds__(kScatterThreads, kScatterCtas) sort_scatter_kernel(const SortParams p) {
@@ -568,7 +568,7 @@ constexpr int kAloneBytes = 116 * 1024;
 constexpr int kCountSmem = 160 * 1024;  // of the counting kernel: a count of every expert for each warp
 
 int sort_chunks(int64_t tokens, int k) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxChunks, tokens * k / 4096));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxChunks, tokens * k / 1024));
 }
 
 template <typename V>
