@@ -151,6 +151,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   __shared__ volatile int abort_flag;
   __shared__ uint32_t tmem_base_shared;
   __shared__ int32_t warp_sums[kThreads / 32];
+  __shared__ long long warp_rows[kThreads / 32];
 
   const int tid = threadIdx.x;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -199,11 +200,13 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   }
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  // The tables: a run of experts to a thread, then a prefix over threads.
+  // The tables: a run of experts to a thread, then a prefix over threads.  Offsets that give more rows than there are would
+  // name tiles without end: nothing is computed then, and the record says so.
   {
     const int each = (p.experts + kThreads - 1) / kThreads;
     const int lo = min(p.experts, tid * each), hi = min(p.experts, lo + each);
     int own = 0;
+    long long rows = 0;
     for (int e = lo; e < hi; ++e) {
       const int from = min(max(__ldcg(p.offsets + e), 0), p.M);
       const int to = min(max(__ldcg(p.offsets + e + 1), from), p.M);
@@ -211,6 +214,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       tables.count[e] = to - from;
       own += (to - from + kBt - 1) / kBt * p.n_tiles;
       tables.tiles_end[e] = own;
+      rows += to - from;
     }
     int upto = own;
 #pragma unroll
@@ -218,11 +222,19 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, o);
     if (lane == 31) warp_sums[warp] = upto;
+    if (lane == 0) warp_rows[warp] = rows;
     __syncthreads();
     int before = upto - own;
     for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    for (int e = lo; e < hi; ++e) tables.tiles_end[e] += before;
+    rows = 0;
+    for (int w = 0; w < kThreads / 32; ++w) rows += warp_rows[w];
+    const bool bad = rows > p.M;
+    for (int e = lo; e < hi; ++e) tables.tiles_end[e] = bad ? 0 : tables.tiles_end[e] + before;
+    if (bad && blockIdx.x == 0 && tid == 0 && p.status != nullptr)
+      store_status(p.status, STATUS_BAD_INDEX, PHASE_NONE, -1, p.experts, 0, (uint64_t)rows);
   }
   ptx::tcgen05_fence_before();
   __syncthreads();

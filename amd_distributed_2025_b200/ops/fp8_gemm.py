@@ -84,7 +84,8 @@ def fp8_grouped_gemm(
     decreasing (``sort_tokens(...).order.offsets``); experts may have no rows.  Returns bf16 ``[M, N]``.  Rows that no
     expert has behind ``offsets[E]`` are zero, or, in a ``c`` that is given, left as they were.
 
-    Expired waits are reported as those of ``fp8_gemm`` are: by ``check()`` or the next call on the device."""
+    Expired waits are reported as those of ``fp8_gemm`` are, by ``check()`` or the next call on the device, and so are
+    offsets that give the experts more rows than there are (nothing is computed then)."""
     ext = _ext.load()
     while True:
         out = ext.fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c, int(timeout_ms * 1e6))

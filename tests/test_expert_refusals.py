@@ -125,3 +125,20 @@ def test_fp8_grouped_gemm_refusals():
     _refused("c must", lambda: f(a, b, sa, sb, off, F(130, 4, dtype=torch.bfloat16).t()))
     _refused("timeout_ms", lambda: f(a, b, sa, sb, off, timeout_ms=0))
     _refused("CUDA", lambda: f(a, b, sa, sb, off))
+
+
+def test_grouped_product_leaves_no_room_for_a_cta_that_waits_for_tensor_memory():
+    """Its CTAs hold all of an SM's tensor memory: none of the GEMM kernels' may fit beside one by shared memory."""
+    from amd_distributed_2025_b200.ops import _ext
+
+    ext = _ext.load()
+    others = [ext.gemm_tile_share(rows, bn, splits, pair)[0] for rows in range(8, 129, 8) for bn in range(32, 257, 32)
+              for pair in (False, True) for splits in range(1, (8 if pair else 16) + 1)]
+    others += [ext.gemm_pair_share(bn, 1)[0] for bn in range(32, 257, 32)] + [ext.gemm_pair_share(256, 2)[0]]
+    others += [ext.gemm_rs_share(bn, pair)[0] for bn, pair in ((64, False), (128, False), (256, False), (128, True), (192, True), (256, True))]
+    others += [ext.fp8_gemm_share(bn, splits)[0] for bn in (64, 128) for splits in range(1, 9)]
+    own = [ext.fp8_grouped_share(tile, experts) for tile in (64, 256) for experts in (1, 7, 256, 1000, 1024)]
+    sm, reserved = 228 * 1024, 1024
+    for smem, columns in own:
+        assert columns == 512 and smem <= 232448
+        assert smem + reserved + min(others + [s for s, _ in own]) + reserved > sm

@@ -657,7 +657,9 @@ def test_fp8_grouped_gemm_matches_fp8_gemm():
 
 
 def test_fp8_grouped_gemm_rows_of_no_expert():
+    from amd_distributed_2025_b200.ops import fp8_gemm as f
     from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+    from amd_distributed_2025_b200.utils.status import StatusError
 
     for n in (264, 129):
         a, b, a_scale, b_scale, offsets = _grouped_inputs([40, 0, 30, 50], n, 256)
@@ -672,8 +674,14 @@ def test_fp8_grouped_gemm_rows_of_no_expert():
         assert torch.equal(given[:70], want[:70]) and bool((given[70:] == 7).all())
         none = torch.zeros_like(offsets)
         assert bool((fp8_grouped_gemm(a, b, a_scale, b_scale, none) == 0).all())
-        # offsets that are no order at all stay inside the matrices
-        fp8_grouped_gemm(a, b, a_scale, b_scale, torch.tensor([-5, 2 ** 31 - 1, -2 ** 31, 90, 400], dtype=torch.int32, device="cuda"))
+        # offsets that are no order at all: more rows than there are is refused, fewer stay inside the matrices
+        wild = torch.tensor([-5, 2 ** 31 - 1, -2 ** 31, 90, 400], dtype=torch.int32, device="cuda")
+        f.fp8_grouped_gemm(a, b, a_scale, b_scale, wild)
+        with pytest.raises(StatusError, match="bad_index"):
+            f.check()
+        f.fp8_grouped_gemm(a, b, a_scale, b_scale, torch.tensor([-5, 40, 10, 5, 60], dtype=torch.int32, device="cuda"))
+        f.check()
+        assert torch.equal(fp8_grouped_gemm(a, b, a_scale, b_scale, fewer)[:70], want[:70])
     empty = _grouped_inputs([0, 0], 64, 128)
     assert fp8_grouped_gemm(*empty).shape == (0, 64)
 
