@@ -779,3 +779,82 @@ def test_experts_of_a_layer_together():
         graph.replay()
         assert torch.equal(captured, layer()[-1])
     check()
+
+
+# --------------------------------------------------------------------------------------
+# more than 2^31 elements, and calls at the same time
+# --------------------------------------------------------------------------------------
+
+def test_rows_beyond_32_bit_offsets():
+    """4.6 GB of rows: their first and last ones, and those about 2^31 elements and 2^32 bytes."""
+    from amd_distributed_2025_b200.ops import fp8_rows, moe_sort
+
+    tokens, k, experts, hidden = 35000, 8, 64, 8192
+    entries = tokens * k
+    assert entries * hidden > 2 ** 31
+    x = _randn(tokens, hidden, dtype=torch.bfloat16, seed=1)
+    ids = _ids(tokens, k, experts, 2)
+    got = moe_sort.sort_tokens(x, ids, experts)
+    offsets, row_of = _order_of(ids, experts)
+    assert torch.equal(got.order.offsets, offsets) and torch.equal(got.order.row_of, row_of)
+    for j in range(k):
+        assert torch.equal(got.rows[row_of[:, j].long()], x)
+    some = torch.cat([torch.arange(0, 40), torch.arange(tokens - 40, tokens)]).cuda()
+    edge = 2 ** 31 // hidden
+    last = torch.cat([torch.arange(0, 40), torch.arange(edge - 20, edge + 20), torch.arange(entries - 40, entries)]).cuda()
+    weights = torch.rand(tokens, k, device="cuda", generator=_gen(3))
+    _check_unsort(got.rows, row_of[some], weights[some], moe_sort.unsort_tokens(got.rows, got.order, weights)[some])
+    grad_rows, grad_weights = moe_sort.unsort_tokens_backward(x, got.rows, got.order, weights)
+    at = torch.empty(entries, dtype=torch.long, device="cuda")  # the entry of a row
+    at[row_of.reshape(-1).long()] = torch.arange(entries, device="cuda")
+    want = x[at[last] // k].double() * weights.reshape(-1)[at[last]].double()[:, None]
+    _close(grad_rows[last], want, (_u(torch.bfloat16) + U32) * want.abs())
+    dot = (x[some].double()[:, None] * got.rows[row_of[some].long()].double()).sum(2)
+    size = (x[some].double()[:, None] * got.rows[row_of[some].long()].double()).abs().sum(2)
+    _close(grad_weights[some], dot, (hidden + 2) * U32 * size)
+    del grad_rows
+    w = torch.ones(hidden, dtype=torch.bfloat16, device="cuda")
+    normed = fp8_rows.rms_norm_fp8(got.rows, w, residual=got.rows)
+    _check_norm(got.rows[last], w, got.rows[last], fp8_rows.NormedRows(normed.q[last], normed.scale[last], normed.total[last], None))
+    del normed
+    wide = got.rows.view(entries // 2, 2 * hidden)
+    last = last[last < entries // 2]
+    last = torch.cat([last, torch.arange(entries // 2 - 40, entries // 2, device="cuda")])
+    q, scale = fp8_rows.silu_mul_fp8(wide)
+    _check_silu(wide[last], (q[last], scale[last]))
+
+
+def test_fp8_grouped_gemm_beyond_32_bit_offsets():
+    from amd_distributed_2025_b200.ops.fp8_gemm import check, fp8_grouped_gemm
+
+    rows, n, k = 140000, 16384, 16
+    assert rows * n > 2 ** 31
+    a, b, a_scale, b_scale, offsets = _grouped_inputs([100, 130900, 9000], n, k)
+    out = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+    check()
+    assert int(offsets[-1]) == rows
+    edge = 2 ** 31 // n
+    for lo, hi, e in ((0, 100, 0), (edge - 40, edge, 2), (edge, edge + 40, 2), (rows - 40, rows, 2), (130900, 131000, 1)):
+        own = torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda")
+        assert int(offsets[e]) <= lo and hi <= int(offsets[e + 1])
+        _check_grouped((a[lo:hi], b[e:e + 1], a_scale[lo:hi], b_scale[e:e + 1], own), out[lo:hi])
+
+
+def test_expert_products_on_two_streams_at_once():
+    """Both kernels (few rows an expert, many), which hold all of an SM's tensor memory, beside one another and fp8_gemm."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import check, fp8_gemm, fp8_grouped_gemm
+
+    few, many = _grouped_inputs([5] * 40, 1024, 2048), _grouped_inputs([700, 30, 1500], 1024, 1024, 2)
+    one = (many[0], many[1][0], many[2], many[3][0])
+    want = fp8_grouped_gemm(*few), fp8_grouped_gemm(*many), fp8_gemm(*one)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(20):
+        for stream, call in zip(streams, (lambda: fp8_grouped_gemm(*few), lambda: fp8_grouped_gemm(*many), lambda: fp8_gemm(*one))):
+            with torch.cuda.stream(stream):
+                got.append(call())
+    torch.cuda.synchronize()
+    check()
+    for i, c in enumerate(got):
+        assert torch.equal(c, want[i % 3])
