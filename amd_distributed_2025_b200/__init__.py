@@ -6,6 +6,7 @@ Public entry points
 -------------------
 ``amd_distributed_2025_b200.models.moe_all2all.custom_kernel(data)``
 ``amd_distributed_2025_b200.models.gemm_rs.custom_kernel(data)``
+``amd_distributed_2025_b200.ops.fp8_gemm``, ``.ops.fp8_rows``, ``.ops.moe_sort`` -- operators around one GPU's experts
 ``amd_distributed_2025_b200.contract`` -- configs, input generators, shape lists
 ``amd_distributed_2025_b200.oracle`` -- communication-free ground truth and checkers
 ``amd_distributed_2025_b200.harness.eval`` -- multi-rank test / benchmark runner

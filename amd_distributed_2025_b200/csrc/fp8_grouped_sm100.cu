@@ -17,9 +17,10 @@
 // fp32 registers while the other is being filled.  Pairs are persistent, and walk the same list of tiles: experts in order,
 // an expert's weight tiles in order, its token tiles innermost, so that pairs at work at the same time share weights in L2.
 //
-// What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 537 us, 7.0
-// TB/s in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x 4096, one expert: 123 us
-// both, 2.2 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights) is between the two, 480 us.
+// What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 535 us, 7.0
+// TB/s in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x 4096, one expert: 122 us,
+// 121 there, 2.25 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights) is between the two:
+// 480 us on one set of inputs, 545 to 586 where every call has its own.
 // What it took, us at 8192 rows of one expert / of 64 experts / at 256 experts with 4 rows each:
 //   tokens always on the free side, up to 256 of them, 16 x 256 bits           154 / 232 / 570
 //   the next piece out of tensor memory while one is added up                  176 / 208 / 552   (registers spill)
@@ -100,7 +101,7 @@ struct Tables {
 };
 
 // A pair's tiles: dealt out in turn, every other round the other way round.  Were it always the same, the token tiles of
-// experts with 384 rows each, 256 and 128, would go to even and to odd pairs for good (64 of them: 533 us, 412).  (A tile from
+// experts with 384 rows each, 256 and 128, would go to even and to odd pairs for good (64 of them: 533 us, 412 to 420).  (A tile from
 // the front of the list and one from its end in turn, or a run of it to each pair, evens out as much and takes L2 its sense:
 // skewed routing 493 and 645 us against 480.)
 template <int BT>
