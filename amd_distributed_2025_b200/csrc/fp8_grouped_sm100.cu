@@ -15,12 +15,12 @@
 // Every 128-wide K block is multiplied into tensor memory of its own: two buffers of 256 columns, each for one K block (256
 // tokens), two (128) or four.  Eight epilogue warps, two to a lane quarter, take a buffer out, hand it back, and add it up in
 // fp32 registers while the other is being filled.  Pairs are persistent, and walk the same list of tiles: experts in order,
-// an expert's weight tiles in order, its token tiles innermost, so that pairs at work at the same time share weights in L2.
+// an expert's in bands, so that pairs at work at the same time share weights and tokens in L2.
 //
 // What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 535 us, 7.0
 // TB/s in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x 4096, one expert: 122 us,
 // 121 there, 2.25 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights) is between the two:
-// 480 us on one set of inputs, 545 to 586 where every call has its own.
+// 478 us at first, 535 to 570 where calls follow on one another for a second: power, at 1.3 to 1.4 GHz.
 // What it took, us at 8192 rows of one expert / of 64 experts / at 256 experts with 4 rows each:
 //   tokens always on the free side, up to 256 of them, 16 x 256 bits           154 / 232 / 570
 //   the next piece out of tensor memory while one is added up                  176 / 208 / 552   (registers spill)
@@ -28,6 +28,7 @@
 //   16 x 128 bits instead (the tensor memory gives those four times as fast)   127 / 221 / 537
 //   buffers emptied at once and handed back before the sums                    120 / 220 / 537
 //   128 tokens as rows                                                         123 / 200 / 537
+//   bands, the epilogue told its tiles                                         122 / 200 / 537   (24576 skewed rows: 491 to 478)
 // Shared memory is what the free side runs short of: sixteen-byte reads take four passes each beside what the tensor cores
 // read (920 cycles for the sums of a buffer that take 240 without them; asked for a half ahead, 650).  A spilled register in
 // the loop costs more the more shared memory is taken, as L1 is what is left of it.  L2 prefetches of weights ahead of the
@@ -68,7 +69,10 @@ constexpr uint32_t kBufCols = 256;
 constexpr int kGroup = 4;       // K blocks whose scales come in together
 constexpr int kScaleSlots = 4;
 constexpr int kSlabBytes = 2048;  // per epilogue warp: 32 tokens x 32 output columns
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 512;  // barriers, and behind them what tiles are
+constexpr int kNotes = 8, kNotesAt = 256;
+static_assert(8 * (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots) <= kNotesAt && kNotesAt + 16 * kNotes <= kBarBytes);
+static_assert(kNotes > kScaleSlots + 1, "a tile has a slot of scales at least: no note is written over that is still read");
 constexpr int kMaxDynamicSmem = 232448 - 256;
 constexpr int kTmemCols = 512;
 constexpr int kBigBox = 64, kSmallBox = 16;  // rows of a copy of tokens
@@ -100,14 +104,20 @@ struct Tables {
   int32_t *start, *count, *tiles_end;
 };
 
+// The list: experts in order, an expert's token tiles in bands of at most kBand (all about as wide), a band's weight tiles in
+// order, its token tiles innermost.  What pairs at work at the same time read is then small next to what they multiply, as in
+// fp8_gemm: without bands the one expert of 24576 rows takes 414 us instead of 364, 476 instead of 414 where calls follow on
+// one another for a second, and power is what there is too little of.
+//
 // A pair's tiles: dealt out in turn, every other round the other way round.  Were it always the same, the token tiles of
-// experts with 384 rows each, 256 and 128, would go to even and to odd pairs for good (64 of them: 533 us, 412 to 420).  (A tile from
-// the front of the list and one from its end in turn, or a run of it to each pair, evens out as much and takes L2 its sense:
-// skewed routing 493 and 645 us against 480.)
+// experts with 384 rows each, 256 and 128, would go to even and to odd pairs for good (64 of them: 533 us, 412 to 420).
+// (A tile from the front of the list and one from its end in turn, or a run of it to each pair, evens out as much and takes
+// L2 its sense: skewed routing 493 and 645 us against 480 then.)
+constexpr int kBand = 8;
 template <int BT>
 struct Walk {
   Tables t;
-  int experts;
+  int experts, n_tiles;
   // The pair's tile of a round, or -1 behind the last.
   __device__ __forceinline__ int tile_of(int round) const {
     const int pairs = (int)gridDim.x >> 1, pair = (int)blockIdx.x >> 1;
@@ -126,8 +136,15 @@ struct Walk {
     const int parts = (count + BT - 1) / BT;
     Tile r;
     r.expert = e;
-    r.nt = local / parts;
-    const int part = local - r.nt * parts;
+    int part = 0;
+    r.nt = local;
+    if (parts > 1) {
+      const int bands = (parts + kBand - 1) / kBand, wide = (parts + bands - 1) / bands;
+      const int band = local / (wide * n_tiles), in_band = local - band * wide * n_tiles;
+      const int of_band = min(wide, parts - band * wide);
+      r.nt = in_band / of_band;
+      part = band * wide + in_band - r.nt * of_band;
+    }
     r.row0 = t.start[e] + part * BT;
     r.rows = min(BT, count - part * BT);
     r.width = BT == 64 ? (r.rows + kChunk - 1) / kChunk * kChunk : r.rows > kRows ? 2 * kRows : kRows;
@@ -173,6 +190,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   auto tfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + s); };
   auto tempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + kBufs + s); };
   auto sfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + s); };
+  auto note = [&](int round) { return bars + (uint32_t)(kNotesAt + round % kNotes * 16); };
   auto sempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + kScaleSlots + s); };
 
   if (tid == 0) {
@@ -242,7 +260,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   ptx::cluster_sync_all();
   ptx::tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_shared;
-  const Walk<kBt> walk{tables, p.experts};
+  const Walk<kBt> walk{tables, p.experts, p.n_tiles};
   // K blocks that are multiplied into a tensor-memory buffer one beside the other.
   auto steps = [](int width) { return WIDE ? 2 * kRows / width : 4; };
 
@@ -345,6 +363,8 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         const float* b0 = bs + min(t.nt * 2 + (WIDE ? 0 : cta), last) * p.bs_stride_n;
         const float* b1 = bs + min(t.nt * 2 + 1, last) * p.bs_stride_n;
         const int token0 = WIDE ? cta * (t.width / 2) : 0;
+        // WIDE: the epilogue is told what the tile is, with the tile's first scales.  It bounds the kernel, and working out its
+        // tiles itself, twice each, took it 2 to 3 % of its time.
         for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
           float s[2][kGroup];
 #pragma unroll
@@ -371,6 +391,9 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
           }
           if (!fp8_wait(sempty_bar(slot), phase ^ 1u, &abort_flag, p, 500 + (int)slot)) break;
           const uint32_t at = scales + slot * kSlotBytes;
+          if (WIDE && kb == 0 && l == 0)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(note(round)), "r"(t.nt), "r"(t.row0), "r"(t.rows), "r"(t.width)
+                         : "memory");
           auto put = [&](int place, const float* f, const float* w) {
 #pragma unroll
             for (int i = 0; i < kGroup; ++i)
@@ -460,8 +483,17 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       }
       __syncwarp();
     };
+    auto noted = [&](int round) {
+      Tile t;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(t.nt), "=r"(t.row0), "=r"(t.rows), "=r"(t.width)
+                   : "r"(note(round))
+                   : "memory");
+      return t;
+    };
     for (int round = 0, tile; (tile = walk.tile_of(round)) >= 0 && !abort_flag; ++round) {
-      const Tile t = walk.at(tile);
+      if (WIDE) await_scales();
+      const Tile t = WIDE ? noted(round) : walk.at(tile);
       if (WIDE && t.width == 2 * kRows) {
         // ---- tokens in lanes: a lane's scale is its token's times that of its columns' block of weights -------
         // A CTA has 128 of 256 tokens in its lanes; `side` is the block of weights.
@@ -505,7 +537,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
         if (!idle) {
-          const Tile t = walk.at(tile);  // (worked out again: what it takes to keep it through the loop is needed there)
+          const Tile t = noted(round);  // (again: what it takes to keep it through the loop is needed there)
           const int first = cta * kRows + q * 32, rows = t.rows - first, n0 = t.nt * 2 * kRows + side * kRows;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -568,7 +600,7 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
         if (!idle) {
-          const Tile t = walk.at(tile);
+          const Tile t = noted(round);
           const int first = cta * (kRows / 2) + (q & 1) * 32, rows = t.rows - first;
           const int n0 = t.nt * 2 * kRows + (q >> 1) * kRows + side * 64;
 #pragma unroll
