@@ -54,12 +54,14 @@ __device__ __forceinline__ void store_vec<Vec32>(Vec32* p, const Vec32& v) {
                : "memory");
 }
 
+constexpr int kMaxChunks = 256;  // runs of tokens that are counted
+
 struct SortParams {
   SortTokensArgs a;
   int32_t pieces;      // of a row
   int32_t row_vecs, piece_vecs;
   int32_t vec_ids;               // 1: ids begin at a multiple of 16 bytes
-  int32_t chunks, chunk_tokens;  // two launches: runs of tokens that are counted by a CTA each
+  int32_t chunks, chunk_tokens;  // several launches: runs of tokens that are counted by a CTA each
 };
 
 __device__ __forceinline__ int checked_id(long long e, int experts) { return e >= 0 && e < experts ? (int)e : -1; }
@@ -119,6 +121,14 @@ struct Piece {
   V r[Copy<V>::U];
   float s[2];
 };
+__device__ __forceinline__ void load_scales(const SortParams& p, int t, float (&s)[2]) {
+  if (p.a.scale == nullptr) return;
+  const int lane = threadIdx.x & 31;
+  const float* scale = p.a.scale + (int64_t)t * p.a.scale_stride;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 32 * u < p.a.scale_cols) s[u] = __ldcg(scale + lane + 32 * u);
+}
 template <typename V>
 __device__ __forceinline__ void load_piece(const SortParams& p, int t, int piece, Piece<V>& to) {
   const int lane = threadIdx.x & 31;
@@ -128,12 +138,16 @@ __device__ __forceinline__ void load_piece(const SortParams& p, int t, int piece
 #pragma unroll
   for (int u = 0; u < Copy<V>::U; ++u)
     if (v0 + 32 * u < v1) to.r[u] = load_vec(src + v0 + 32 * u);
-  if (piece == 0 && p.a.scale != nullptr) {
-    const float* scale = p.a.scale + (int64_t)t * p.a.scale_stride;
+  if (piece == 0) load_scales(p, t, to.s);
+}
+// Token t's scales, to row `to`.
+__device__ __forceinline__ void store_scales(const SortTokensArgs& a, int t, int to, const float (&s)[2]) {
+  const int lane = threadIdx.x & 31;
+  float* scale = a.rows_scale + (int64_t)to * a.scale_cols;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 32 * u < p.a.scale_cols) to.s[u] = __ldcg(scale + lane + 32 * u);
-  }
+  for (int u = 0; u < 2; ++u)
+    if (lane + 32 * u < a.scale_cols) scale[lane + 32 * u] = s[u];
+  for (int c = lane + 64; c < a.scale_cols; c += 32) scale[c] = __ldcg(a.scale + (int64_t)t * a.scale_stride + c);
 }
 // Stores it to the token's k rows; `row` is lane j's: entry j's row.
 template <typename V>
@@ -151,13 +165,7 @@ __device__ __forceinline__ void store_piece(const SortParams& p, int t, int piec
 #pragma unroll
     for (int u = 0; u < Copy<V>::U; ++u)
       if (v0 + 32 * u < v1) store_vec(dst + v0 + 32 * u, from.r[u]);
-    if (scales) {
-      float* scale = a.rows_scale + (int64_t)to * a.scale_cols;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + 32 * u < a.scale_cols) scale[lane + 32 * u] = from.s[u];
-      for (int c = lane + 64; c < a.scale_cols; c += 32) scale[c] = __ldcg(a.scale + (int64_t)t * a.scale_stride + c);
-    }
+    if (scales) store_scales(a, t, to, from.s);
   }
 }
 
@@ -244,9 +252,9 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(const SortParams p) {
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, n, (int)blockIdx.x, (int)gridDim.x);
 }
 
-// Two launches, the first: a CTA counts a run of tokens' entries by expert, and ranks them inside the run.  Warps have runs
-// of their own inside it, so that order needs no other means than a prefix over warps.
-// work: [chunk][expert] counts, then a rank for each entry.
+// Two launches, or three, the first: a CTA counts a run of tokens' entries by expert, and ranks them inside the run.  Warps have
+// runs of their own inside it, so that order needs no other means than a prefix over warps.
+// work: [chunk][expert] counts, [expert] room for their sums, then a rank for each entry.
 __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
   extern __shared__ __align__(16) int32_t smem[];  // [warp][expert]
   const SortTokensArgs& a = p.a;
@@ -260,7 +268,7 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
   const int each = ((i1 - i0 + warps - 1) / warps + 31) & ~31;
   const int w0 = min(i1, i0 + warp * each), w1 = min(i1, w0 + each);
   int32_t* own = smem + warp * a.experts;
-  int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
+  int32_t* ranks = a.work + (int64_t)(p.chunks + 1) * a.experts;
   auto rank_of = [&](int e) {  // among the warp's entries so far (every lane has one, or -1)
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     int rank = 0;
@@ -306,11 +314,11 @@ __global__ void __launch_bounds__(1024) sort_count_kernel(const SortParams p) {
   }
 }
 
-// The second: a CTA adds up the runs' counts, and copies its share of the rows, which lies in one run or two.
+// Rows that are short: a CTA adds up the runs' counts, and copies its share of the rows, which lies in one run or two.
 //
 // Bound by the row stores, which memory takes the slower the more of them are under way in different places: 65536 rows of
-// 7168 bytes with scales (8192 tokens, top-8) take 111 us with 16 to 32 warps an SM, 5 to 8 more with 48, 16 more with 64; as bare
-// copies, without the counting and the scales, 93 to 100.  (Scales as a piece of their own, whose loads wait behind the stores
+// 7168 bytes with scales (8192 tokens, top-8) would take 111 us with 16 to 32 warps an SM, 5 to 8 more with 48, 16 more with 64;
+// as bare copies, without the counting and the scales, 93 to 100.  (Scales as a piece of their own, whose loads wait behind the stores
 // of others: 8 us more.  In the order of the rows instead of the tokens': 115 and more for the copies alone.)
 constexpr int kScatterThreads = 512, kScatterCtas = 2;
 template <typename V>
@@ -355,7 +363,7 @@ __global__ void __launch_bounds__(kScatterThreads, kScatterCtas) sort_scatter_ke
     if (tid == 0) a.offsets[a.experts] = total;
   }
   __syncthreads();
-  const int32_t* ranks = a.work + (int64_t)p.chunks * a.experts;
+  const int32_t* ranks = a.work + (int64_t)(p.chunks + 1) * a.experts;
   int64_t item = lo + (tid >> 5);
   Piece<V> next_piece;
   int next_id = -1, next_rank = 0;
@@ -376,6 +384,132 @@ __global__ void __launch_bounds__(kScatterThreads, kScatterCtas) sort_scatter_ke
     store_piece(p, t, (int)(item - (int64_t)t * P), row, now);
   }
   zero_rows<V>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, (int64_t)a.tokens * a.k, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// Rows that are long, the second launch: for each expert, a run's count becomes that of the runs before it.  Eight warps share
+// the runs of 32 experts.
+__global__ void __launch_bounds__(256) sort_prefix_kernel(const SortParams p) {
+  __shared__ int32_t sums[8][32];
+  const SortTokensArgs& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.x * 32 + lane;
+  const int each = (p.chunks + 7) / 8;
+  const int q0 = min(p.chunks, warp * each), q1 = e < a.experts ? min(p.chunks, q0 + each) : q0;
+  int32_t* counts = a.work + e;
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  constexpr int kHeld = kMaxChunks / 8;
+  int held[kHeld], own = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held[i] = q0 + i < q1 ? __ldcg(counts + (int64_t)(q0 + i) * a.experts) : 0;
+    own += held[i];
+  }
+  sums[warp][lane] = own;
+  __syncthreads();
+  int run = 0;
+  for (int w = 0; w < warp; ++w) run += sums[w][lane];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    if (q0 + i < q1) counts[(int64_t)(q0 + i) * a.experts] = run;
+    run += held[i];
+  }
+  if (warp == 7 && e < a.experts) counts[(int64_t)p.chunks * a.experts] = run;
+}
+
+namespace {
+
+// Entry `lane` of a token on its way to its row: its expert and rank, then what its expert's earlier runs have.
+struct Entry {
+  int id, rank, base;
+  __device__ __forceinline__ void ask(const SortParams& p, int t) {
+    const int lane = threadIdx.x & 31;
+    id = -1;
+    if (lane >= p.a.k) return;
+    id = expert_of(p.a, (int64_t)t * p.a.k + lane);
+    rank = __ldcg(p.a.work + (int64_t)(p.chunks + 1) * p.a.experts + (int64_t)t * p.a.k + lane);
+  }
+  __device__ __forceinline__ void ask_base(const SortParams& p, int t) {
+    if (id >= 0) base = __ldcg(p.a.work + (int64_t)(t / p.chunk_tokens) * p.a.experts + id);
+  }
+  __device__ __forceinline__ int row(const int32_t* start) const { return id >= 0 ? start[id] + base + rank : -1; }
+};
+
+}  // namespace
+
+// The third: a piece of a row comes into shared memory, and leaves it by a bulk copy for each of the token's rows, one to a lane.
+// A warp has room for two pieces: one comes in while the other leaves.  There is one CTA to an SM, and all of them take tokens
+// in order together, so that few rows are written at a time, and near one another inside an expert: as bare copies 90 us for
+// 65536 rows of 7168 bytes, 97 to 99 when each CTA has a share of its own or an SM has two.  With everything, us, beside the
+// kernel above (8192 tokens, top-8, unless said): 7168 bytes and scales 107, 113; 14336 bytes 197, 202; 4096 bytes and scales
+// 66, 69; 2048 bytes 40, 37 (which is why rows have to be long); 5000 tokens of 40000 bytes 336, 365; 9000 tokens, top-4 of
+// 4096, 4112 bytes 52, 71.  With four warps and pieces of 16 KiB long rows take 2 % less, short ones 12 to 17 % more.
+constexpr int kBulkWarps = 8, kBulkPiece = 8192;
+__global__ void __launch_bounds__(32 * kBulkWarps) sort_scatter_bulk_kernel(const SortParams p) {
+  extern __shared__ __align__(128) int32_t smem[];
+  __shared__ int32_t warp_sums[32];
+  const SortTokensArgs& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int P = p.pieces;
+  const uint32_t slot_bytes = (uint32_t)p.piece_vecs * 16u;
+  const uint32_t slots = ptx::smem_u32(smem) + (uint32_t)warp * 2u * slot_bytes;
+  int32_t* start = smem + kBulkWarps * 2 * p.piece_vecs * 4;
+  const int64_t items = (int64_t)a.tokens * P;
+  const int64_t step = (int64_t)gridDim.x * kBulkWarps;
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  int64_t item = (int64_t)warp * gridDim.x + blockIdx.x;
+  Entry entry;
+  float scales[2];
+  auto bring = [&](int64_t i, uint32_t slot) {
+    if (i < items) {
+      const int t = (int)(i / P), v0 = (int)(i - (int64_t)t * P) * p.piece_vecs, n = min(p.piece_vecs, p.row_vecs - v0);
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(a.x) + (int64_t)t * a.x_stride + (int64_t)v0 * 16;
+      for (int v = lane; v < n; v += 32) ptx::cp_async_16(slot + (uint32_t)v * 16u, src + (int64_t)v * 16);
+    }
+    ptx::cp_async_commit();
+  };
+  auto ask = [&](int64_t i) {
+    if (i >= items) return;
+    const int t = (int)(i / P);
+    entry.ask(p, t);
+    if (i % P == 0) load_scales(p, t, scales);
+    entry.ask_base(p, t);
+  };
+  bring(item, slots);
+  ask(item);
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) start[e] = __ldcg(a.work + (int64_t)p.chunks * a.experts + e);
+  __syncthreads();
+  const int total = exclusive_scan(start, a.experts, warp_sums);
+  if (blockIdx.x == 0) {
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) a.offsets[e] = start[e];
+    if (threadIdx.x == 0) a.offsets[a.experts] = total;
+  }
+  for (uint32_t slot = slots, other = slots + slot_bytes; item < items; item += step) {
+    ptx::bulk_wait_group_read<0>();  // the copies out of the other slot have read it
+    __syncwarp();
+    bring(item + step, other);
+    ptx::cp_async_wait_group<1>();
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    const int t = (int)(item / P), piece = (int)(item - (int64_t)t * P), v0 = piece * p.piece_vecs;
+    const int row = entry.row(start);
+    if (row >= 0)
+      ptx::bulk_store(reinterpret_cast<uint8_t*>(a.rows) + (int64_t)row * a.row_bytes + (int64_t)v0 * 16, slot,
+                      (uint32_t)min(p.piece_vecs, p.row_vecs - v0) * 16u);
+    ptx::bulk_commit_group();
+    if (piece == 0 && lane < a.k) a.row_of[(int64_t)t * a.k + lane] = row;
+    for (int j = 0; piece == 0 && a.scale != nullptr && j < a.k; ++j) {
+      const int to = __shfl_sync(0xffffffffu, row, j);
+      if (to >= 0) store_scales(a, t, to, scales);
+    }
+    ask(item + step);
+    const uint32_t done = slot;
+    slot = other;
+    other = done;
+  }
+  ptx::bulk_wait_group<0>();
+  zero_rows<int4>(a.rows, a.row_bytes, a.rows_scale, a.scale_cols, total, (int64_t)a.tokens * a.k, (int)blockIdx.x, (int)gridDim.x);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -561,7 +695,8 @@ __global__ void __launch_bounds__(1024) unsort_tokens_backward_kernel(const Unso
 namespace {
 
 constexpr int64_t kOneLaunchEntries = 32768;
-constexpr int kMaxChunks = 256;
+constexpr int64_t kBulkRow = 4096;  // bytes of a row that is long (figures at the kernel)
+constexpr int kBulkSmem = kBulkWarps * 2 * kBulkPiece;
 // Shared memory that keeps a CTA alone on its SM: where two fit, a launch that starts while the one before it still runs may
 // put two on the SMs that happen to be free, and none on others.
 constexpr int kAloneBytes = 116 * 1024;
@@ -602,14 +737,25 @@ cudaError_t sort_typed(SortParams p, int sms, cudaStream_t stream) {
   p.chunks = (a.tokens + p.chunk_tokens - 1) / p.chunk_tokens;
   static OncePerDevice once;
   const cudaError_t opted = once([] {
-    const cudaError_t e = opt_in(sort_count_kernel, kCountSmem, false);
-    return e != cudaSuccess ? e : opt_in(sort_scatter_kernel<V>, 3 * kSortMaxExperts * (int)sizeof(int32_t), false);
+    cudaError_t e = opt_in(sort_count_kernel, kCountSmem, false);
+    if (e == cudaSuccess) e = opt_in(sort_scatter_kernel<V>, 3 * kSortMaxExperts * (int)sizeof(int32_t), false);
+    if (e == cudaSuccess) e = opt_in(sort_scatter_bulk_kernel, kBulkSmem + kSortMaxExperts * (int)sizeof(int32_t), false);
+    return e;
   });
   if (opted != cudaSuccess) return opted;
   const int warps = std::max(1, std::min(32, kCountSmem / (a.experts * (int)sizeof(int32_t))));
   cudaError_t e = ptx::launch_dependent(sort_count_kernel, p.chunks, 32 * warps, (size_t)warps * a.experts * sizeof(int32_t),
                                         stream, p);
   if (e != cudaSuccess) return e;
+  if (sizeof(V) >= 16 && a.row_bytes >= kBulkRow) {
+    e = ptx::launch_dependent(sort_prefix_kernel, (a.experts + 31) / 32, 256, 0, stream, p);
+    if (e != cudaSuccess) return e;
+    p.row_vecs = (int)(a.row_bytes / 16);
+    p.pieces = (p.row_vecs * 16 + kBulkPiece - 1) / kBulkPiece;
+    p.piece_vecs = (p.row_vecs + p.pieces - 1) / p.pieces;
+    const size_t smem = (size_t)kBulkWarps * 2 * p.piece_vecs * 16 + a.experts * sizeof(int32_t);
+    return ptx::launch_dependent(sort_scatter_bulk_kernel, sms, 32 * kBulkWarps, std::max<size_t>(smem, kAloneBytes), stream, p);
+  }
   // (a share is no longer than a run: there are more CTAs than runs)
   const int grid = (int)std::max<int64_t>(p.chunks, std::min<int64_t>((items + kScatterThreads / 32 - 1) / (kScatterThreads / 32),
                                                                      kScatterCtas * (int64_t)sms));
@@ -670,7 +816,7 @@ cudaError_t backward_vec(const UnsortBackwardArgs& a, int sms, cudaStream_t stre
 
 int64_t sort_tokens_work(int64_t tokens, int k, int experts) {
   if (tokens * k <= kOneLaunchEntries) return 0;
-  return (int64_t)sort_chunks(tokens, k) * experts + tokens * k;
+  return (int64_t)(sort_chunks(tokens, k) + 1) * experts + tokens * k;
 }
 
 cudaError_t launch_sort_tokens(const SortTokensArgs& a, int sms, cudaStream_t stream) {

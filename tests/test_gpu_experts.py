@@ -310,6 +310,23 @@ def test_sort_tokens_e4m3_rows_with_scales(tokens, k, experts, hidden):
     _check_sort(x, ids, experts, sort_tokens(x, ids, experts, scale=wide), wide)
 
 
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "one", "none"])
+@pytest.mark.parametrize("tokens,k,experts,hidden,stride", [(2000, 20, 8192, 4112, 4112), (1100, 32, 3, 4096, 5120), (33001, 1, 5, 4224, 4224),
+                                                            (6000, 7, 64, 20000, 20016), (5000, 8, 65, 4100, 4100), (5000, 7, 200, 24592, 24592)])
+def test_sort_tokens_long_rows(tokens, k, experts, hidden, stride, kind):
+    """More entries than one launch takes, rows of a page and more: e4m3 with scales, then bf16 without."""
+    from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
+
+    x = _randn(tokens, stride, seed=tokens).to(torch.float8_e4m3fn)[:, :hidden]
+    scale = torch.rand(tokens, -(-hidden // 128), device="cuda", generator=_gen(2))
+    for wide in (torch.int32, torch.int64):
+        ids = _ids(tokens, k, experts, 3, kind, wide)
+        _check_sort(x, ids, experts, sort_tokens(x, ids, experts, scale=scale), scale)
+    if hidden % 2 == 0 and stride % 2 == 0:
+        half = x.contiguous().view(torch.bfloat16)
+        _check_sort(half, ids, experts, sort_tokens(half, ids, experts))
+
+
 def test_sort_tokens_strides_alignment_and_wide_ids():
     from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
 
