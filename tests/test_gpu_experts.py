@@ -521,11 +521,11 @@ def test_sort_and_unsort_captured_and_replayed():
     """A training step in a graph: new inputs, the same buffers; twice in one graph, each with results of its own."""
     from amd_distributed_2025_b200.ops import moe_sort
 
-    for tokens in (64, 5000):  # one launch, and two
-        x = _randn(tokens, 128, seed=1).requires_grad_()
+    for tokens, hidden in ((64, 128), (5000, 128), (9000, 128), (9000, 1100)):  # one launch, two, and three
+        x = _randn(tokens, hidden, seed=1).requires_grad_()
         weights = torch.rand(tokens, 4, device="cuda").requires_grad_()
         ids = _ids(tokens, 4, 16, 2, "skewed")
-        grad = _randn(tokens, 128, seed=3)
+        grad = _randn(tokens, hidden, seed=3)
 
         def step():
             got = moe_sort.sort_tokens(x, ids, 16)
@@ -542,7 +542,7 @@ def test_sort_and_unsort_captured_and_replayed():
             first, second = step(), step()
         for seed in (5, 6):
             with torch.no_grad():
-                x.copy_(_randn(tokens, 128, seed=seed))
+                x.copy_(_randn(tokens, hidden, seed=seed))
                 ids.copy_(_ids(tokens, 4, 16, seed, "skewed"))
             graph.replay()
             want = step()
@@ -594,6 +594,24 @@ def test_expert_operators_on_streams_of_their_own():
         want_rows, want_normed = cases[i % 2][2:]
         assert torch.equal(rows.rows, want_rows.rows) and torch.equal(rows.order.row_of, want_rows.order.row_of)
         assert torch.equal(normed.q.view(torch.uint8), want_normed.q.view(torch.uint8)) and torch.equal(normed.total, want_normed.total)
+
+
+def test_long_and_short_rows_sorted_on_two_streams_at_once():
+    """More entries than one launch takes: the launches of one call lie between those of the other."""
+    from amd_distributed_2025_b200.ops.moe_sort import sort_tokens
+
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    cases = [(_randn(9000, hidden, dtype=torch.bfloat16, seed=hidden), _ids(9000, 4, experts, hidden, "skewed"), experts)
+             for hidden, experts in ((2056, 300), (256, 64))]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(sort_tokens(*case))
+    torch.cuda.synchronize()
+    for i, rows in enumerate(got):
+        _check_sort(*cases[i % 2], rows)
 
 
 # --------------------------------------------------------------------------------------
