@@ -28,7 +28,7 @@
 //   16 x 128 bits instead (the tensor memory gives those four times as fast)   127 / 221 / 537
 //   buffers emptied at once and handed back before the sums                    120 / 220 / 537
 //   128 tokens as rows                                                         123 / 200 / 537
-//   bands, the epilogue told its tiles                                         122 / 200 / 537   (24576 skewed rows: 491 to 478)
+//   bands, the epilogue told its tiles                                         122 / 200 / 537   (24576 skewed: 491 to 478)
 // Shared memory is what the free side runs short of: sixteen-byte reads take four passes each beside what the tensor cores
 // read (920 cycles for the sums of a buffer that take 240 without them; asked for a half ahead, 650).  A spilled register in
 // the loop costs more the more shared memory is taken, as L1 is what is left of it.  L2 prefetches of weights ahead of the
@@ -69,8 +69,8 @@ constexpr uint32_t kBufCols = 256;
 constexpr int kGroup = 4;       // K blocks whose scales come in together
 constexpr int kScaleSlots = 4;
 constexpr int kSlabBytes = 2048;  // per epilogue warp: 32 tokens x 32 output columns
-constexpr int kBarBytes = 512;  // barriers, and behind them what tiles are
-constexpr int kNotes = 8, kNotesAt = 256;
+constexpr int kBarBytes = 512;  // barriers, and behind them notes of what tiles are
+constexpr int kNotes = 8, kNotesAt = 256;  // of tiles, 16 bytes each
 static_assert(8 * (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots) <= kNotesAt && kNotesAt + 16 * kNotes <= kBarBytes);
 static_assert(kNotes > kScaleSlots + 1, "a tile has a slot of scales at least: no note is written over that is still read");
 constexpr int kMaxDynamicSmem = 232448 - 256;
@@ -190,8 +190,9 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   auto tfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + s); };
   auto tempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + kBufs + s); };
   auto sfull_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + s); };
-  auto note = [&](int round) { return bars + (uint32_t)(kNotesAt + round % kNotes * 16); };
   auto sempty_bar = [&](uint32_t s) { return bars + 8u * (2 * kMaxStages + 2 * kBufs + kScaleSlots + s); };
+  // What the tile of a round is, for the epilogue.
+  auto note = [&](int round) { return bars + (uint32_t)(kNotesAt + round % kNotes * 16); };
 
   if (tid == 0) {
     abort_flag = 0;
