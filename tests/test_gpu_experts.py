@@ -679,7 +679,7 @@ def test_fp8_grouped_gemm_keeps_its_sums_in_registers():
 
     ext = _ext.load()
     assert [ext.fp8_grouped_local_bytes(tile) for tile in (64, 256)] == [0, 0]
-    assert ext.fp8_grouped_tile(72 * 8 + 7, 8) == 64 and ext.fp8_grouped_tile(73 * 8, 8) == 256
+    assert ext.fp8_grouped_tile(64 * 8 + 7, 8) == 64 and ext.fp8_grouped_tile(65 * 8, 8) == 256
 
 
 def test_fp8_grouped_gemm_matches_fp8_gemm():
