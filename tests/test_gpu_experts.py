@@ -657,6 +657,8 @@ GROUPED = [
     ([4] * 256, 256, 640), ([0] * 100 + [7] + [0] * 155, 512, 2880), ([256], 512, 512), ([257, 255, 300, 129, 1], 264, 400),
     ([1000, 0, 500, 3], 1000, 896), ([70] * 9, 200, 1152), ([97, 200, 10, 0, 96], 640, 384), ([1] * 1024, 64, 128),
     ([5000, 20, 1], 300, 256), ([511, 513], 2048, 1536),
+    ([100] * 7, 320, 1152), ([65, 128, 1, 129, 96, 33, 97, 127], 400, 400), ([0, 0, 350, 0, 1], 513, 272), ([70], 64, 144),
+    ([127, 70] * 40, 256, 896), ([900] + [1] * 8, 264, 640),
     ([2400, 100, 4700], 600, 128), ([700] + [0] * 14 + [9], 600, 384), ([4353], 513, 144),
 ]
 
