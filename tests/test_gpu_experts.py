@@ -896,3 +896,69 @@ def test_expert_products_on_two_streams_at_once():
     check()
     for i, c in enumerate(got):
         assert torch.equal(c, want[i % 3])
+
+
+# --------------------------------------------------------------------------------------
+# block scales to the last bit
+# --------------------------------------------------------------------------------------
+
+def _check_quotients(q, scale, y):
+    """y is the kernel's own fp32 matrix: scales are to a step of it, a product with 1/448 (rounded, both), and values are its
+    quotients by them, rounded as a division is and then to e4m3."""
+    rows, cols = y.shape
+    blocks = -(-cols // 128)
+    padded = torch.nn.functional.pad(y, (0, blocks * 128 - cols)).view(rows, blocks, 128)
+    want = padded.double().abs().amax(2).clamp(min=1e-30) / 448
+    _close(scale, want, (2 * U32 + U32 ** 2) * want, "scale")
+    values = (padded / scale[:, :, None]).view(rows, -1)[:, :cols].to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), values.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("cols", [2048, 264, 1001])
+def test_fp8_values_are_quotients_by_their_scale(cols):
+    """Values between two e4m3 numbers too: whole numbers times one factor have many of those."""
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8, silu_mul_fp8
+
+    rows = 3000
+    whole = torch.randint(-448, 449, (rows, cols), device="cuda", generator=_gen(1)).float()
+    for x, w in ((whole, torch.exp2(torch.randint(-3, 4, (cols,), device="cuda", generator=_gen(2)).float())),
+                 (_randn(rows, cols, seed=3), 1 + 0.2 * _randn(cols, seed=4))):
+        got = rms_norm_fp8(x, w, normed=True)  # (fp32: the normed rows are what was quantised)
+        _check_quotients(got.q, got.scale, got.normed)
+        for dtype in DTYPES:  # 32 / (1 + exp(-32)) is 32, so the products are known
+            values = x.to(dtype)
+            _check_quotients(*silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1)), values.float() * 32)
+
+
+@pytest.mark.parametrize("cols", [2048, 264, 1001])
+def test_fp8_blocks_at_both_ends_of_the_range(cols):
+    """Largest values from 2^126, whose reciprocal is no normal number, up to the largest finite one, and small ones."""
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8, silu_mul_fp8
+
+    rows = 64
+    top = torch.finfo(torch.float32).max
+    y = torch.rand(rows, cols, device="cuda", generator=_gen(1)) * 2 - 1
+    sizes = torch.logspace(-37.9, 38.5, rows, device="cuda", dtype=torch.float64)
+    sizes[-8:] = torch.tensor([2.0 ** 126, 1.1 * 2.0 ** 126, 2.0 ** 127, 1.9 * 2.0 ** 127, top, 1e38, 2e38, 3e38], dtype=torch.float64)
+    y = (y.double() * sizes[:, None]).float()
+    y[:, ::200] = sizes.float().clamp(max=top)[:, None]
+    values = y / 32
+    products = values * 32
+    assert bool(products.isfinite().all())
+    _check_quotients(*silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1)), products)
+    got = rms_norm_fp8(_randn(rows, cols, seed=5), torch.full((cols,), 5e37, device="cuda"), normed=True)
+    assert bool(got.normed.isfinite().all()) and bool((got.normed.abs().amax(1) > 2.0 ** 126).any())
+    _check_quotients(got.q, got.scale, got.normed)
+
+
+def test_fp8_zeros_keep_their_signs():
+    from amd_distributed_2025_b200.ops.fp8_rows import silu_mul_fp8
+
+    values = torch.zeros(2, 512, device="cuda")
+    values[:, ::2] = -0.0
+    values[1, 5], values[1, 200] = 1.0, float("inf")
+    _check_quotients(*silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1)[:1]), values[:1] * 32)
+    q, scale = silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1))
+    raw = q[1].view(torch.uint8)
+    assert raw[4] == 0x80 and raw[7] == 0 and raw[5] == 0x7E and bool(scale[1, 1].isinf())
+    assert raw[202] == 0x80 and raw[201] == 0 and bool(q[1, 200].float().isnan())  # over infinity: zeros
