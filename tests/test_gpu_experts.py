@@ -962,3 +962,19 @@ def test_fp8_zeros_keep_their_signs():
     raw = q[1].view(torch.uint8)
     assert raw[4] == 0x80 and raw[7] == 0 and raw[5] == 0x7E and bool(scale[1, 1].isinf())
     assert raw[202] == 0x80 and raw[201] == 0 and bool(q[1, 200].float().isnan())  # over infinity: zeros
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_silu_mul_fp8_gates_whose_exponential_is_near_the_end_of_the_range(dtype):
+    """exp(-gate) from 2^115 to 2^128, times values so large that the product counts."""
+    from amd_distributed_2025_b200.ops.fp8_rows import silu_mul_fp8
+
+    for cols in (256, 250):
+        gates = torch.linspace(-88.5, -80, 17, device="cuda").to(dtype)[:, None].expand(17, cols)
+        values = ((torch.rand(17, cols, device="cuda", generator=_gen(1)) * 2 - 1) * 3e38).to(dtype)
+        x = torch.cat([gates, values], 1)
+        g, u = gates.double(), values.double()
+        y = g / (1 + torch.exp(-g)) * u
+        assert bool((y.abs().amax(1) > 1e-2).all())
+        # as _check_silu; below 2^-126 the exponential has at least 21 bits
+        _check_quantised(*silu_mul_fp8(x), y, (88.5 * 1.5 + 8) * U32 + 2.0 ** -21)
