@@ -12,7 +12,7 @@
 // million quotients, a third of them within two steps of a border between two e4m3 values, all come out as a division's
 // do; the product alone sends 2.8 million to the other side.  What the step takes, us: 16384 x 4096 bf16 73 as before with a
 // residual, 48 to 51 without (with rounded reciprocals, value by value, 55); activation, 32761 x 2048 bf16, 52 to 53, and 50
-with its gates in pairs too.
+// with its gates in pairs too.
 //
 // A lane holds 16 neighbouring columns of a block (eight lanes to a block) where rows are whole aligned 32-byte pieces, eight
 // (sixteen lanes) where they are 16-byte pieces, else every 32nd column (a warp to a block), so that 2-byte loads and
