@@ -156,7 +156,7 @@ PyObject* silu_mul_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {  // (x) ->
     count_args(n, 1);
     const at::Tensor& x_in = tensor_arg(v[0]);
     TORCH_CHECK(x_in.dim() == 2, "x must be a matrix [rows, 2 columns]");
-    TORCH_CHECK(x_in.size(1) >= 2 && x_in.size(1) % 2 == 0 && x_in.size(1) / 2 <= INT32_MAX - 256,
+    TORCH_CHECK(x_in.size(1) >= 2 && x_in.size(1) % 2 == 0 && x_in.size(1) / 2 <= b200::kMaxSiluCols,
                 "x must have an even number of columns: gates, then the values that they multiply");
     const int64_t rows = x_in.size(0), cols = x_in.size(1) / 2;
     const int code = dtype_code(x_in.scalar_type());

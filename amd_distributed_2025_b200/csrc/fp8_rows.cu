@@ -336,12 +336,13 @@ __global__ void __launch_bounds__(256) silu_mul_fp8_kernel(const SiluMulFp8Args 
   const int blocks = (p.cols + kBlockCols - 1) / kBlockCols;
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  // all lanes of a warp make the same number of rounds: they meet in the maximum
+  // All lanes of a CTA make the same number of rounds, over units behind the row as well: a warp's meet in the maximum.
   for (int64_t row0 = (int64_t)blockIdx.x * blockDim.y; row0 < p.rows; row0 += (int64_t)gridDim.x * blockDim.y) {
     const int64_t row = row0 + threadIdx.y;
     const int cols = row < p.rows ? p.cols : 0;
     const T* gate = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
-    for (int u = (int)threadIdx.x; u < blocks * L::kUnits; u += lanes) {
+    for (int u0 = 0; u0 < blocks * L::kUnits; u0 += lanes) {
+      const int u = u0 + (int)threadIdx.x;
       const auto rg = L::load(gate, u, cols), ru = L::load(gate + p.cols, u, cols);
       float g[PER], v[PER];
       L::floats(rg, g);
@@ -431,7 +432,7 @@ cudaError_t norm_weight(const RmsNormFp8Args& p, int sms, cudaStream_t stream) {
 
 template <typename T, int PER>
 cudaError_t silu_units(const SiluMulFp8Args& p, int sms, cudaStream_t stream) {
-  const int units = (p.cols + kBlockCols - 1) / kBlockCols * Lanes<PER>::kUnits;
+  const int64_t units = (int64_t)((p.cols + kBlockCols - 1) / kBlockCols) * Lanes<PER>::kUnits;
   // the largest team of which no more than a ninth is idle
   int lanes = Lanes<PER>::kUnits;
   for (int l = 2 * lanes; l <= 256; l *= 2)
@@ -464,7 +465,7 @@ cudaError_t launch_rms_norm_fp8(const RmsNormFp8Args& p, int sms, cudaStream_t s
 }
 
 cudaError_t launch_silu_mul_fp8(const SiluMulFp8Args& p, int sms, cudaStream_t stream) {
-  if (p.rows < 0 || p.cols < 1) return cudaErrorInvalidValue;
+  if (p.rows < 0 || p.cols < 1 || p.cols > kMaxSiluCols) return cudaErrorInvalidValue;
   if (p.rows == 0) return cudaSuccess;
   switch (p.dtype) {
     case 0: return silu_typed<__half>(p, sms, stream);

@@ -6,6 +6,7 @@
 namespace b200 {
 
 constexpr int kMaxNormCols = 32768;  // a row is held in the registers of one CTA
+constexpr int kMaxSiluCols = INT32_MAX - 8192;  // (a team's last round may reach up to 4096 columns behind a row's last block)
 
 // dtype: 0 fp16, 1 bf16, 2 fp32 (x, residual, total, normed; the weight has its own).  Rows are contiguous; strides in
 // elements from row to row.  q [rows, cols] and scale [rows, ceil(cols / 128)] are contiguous.

@@ -978,3 +978,15 @@ def test_silu_mul_fp8_gates_whose_exponential_is_near_the_end_of_the_range(dtype
         assert bool((y.abs().amax(1) > 1e-2).all())
         # as _check_silu; below 2^-126 the exponential has at least 21 bits
         _check_quantised(*silu_mul_fp8(x), y, (88.5 * 1.5 + 8) * U32 + 2.0 ** -21)
+
+
+@pytest.mark.parametrize("cols", [1032, 1040, 1152, 1408, 2816, 2880, 2888, 8976])
+def test_silu_mul_fp8_rows_whose_last_round_leaves_part_of_a_warp_idle(cols):
+    """Rows of a few units more than whole rounds of a team: its warps stay together, and nothing behind a row is written."""
+    from amd_distributed_2025_b200.ops.fp8_rows import silu_mul_fp8
+
+    for rows in (1, 3, 333):
+        for dtype in DTYPES:
+            values = _randn(rows, cols, dtype=dtype, seed=rows)
+            q, scale = silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1))
+            _check_quotients(q, scale, values.float() * 32)
