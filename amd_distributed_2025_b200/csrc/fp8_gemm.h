@@ -43,7 +43,7 @@ struct Fp8GroupedArgs {
   void* c;                // [M, N] bf16 row-major
   int M, N, K, experts;
   long long as_stride_m, as_stride_k, bs_stride_e, bs_stride_n, bs_stride_k;  // element strides of the scale tensors
-  bool zero_rest;         // rows of C behind offsets[E] are zeroed, else left as they were
+  bool zero_rest;         // rows of C in front of offsets[0] and behind offsets[E] are zeroed, else left as they were
   uint64_t timeout_ns;
   StatusWord* status;
   int sms;

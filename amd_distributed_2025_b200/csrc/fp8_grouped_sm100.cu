@@ -701,10 +701,10 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
       }
       send(t.row0 + token0, t.rows - token0, n0);
     }
-    if (p.zero_rest) {  // rows of no expert, a row to a warp
-      const int end = min(max(__ldcg(p.offsets + p.experts), 0), p.M);
-      for (int row = end + (int)blockIdx.x * kEpiWarps + ew; row < p.M; row += (int)gridDim.x * kEpiWarps) {
-        __nv_bfloat16* c = p.c + (long long)row * p.N;
+    if (p.zero_rest) {  // rows of no expert, in front of the first one's and behind the last one's, a row to a warp
+      const int front = tables.start[0], behind = tables.start[p.experts - 1] + tables.count[p.experts - 1];
+      for (int i = (int)blockIdx.x * kEpiWarps + ew; i < front + p.M - behind; i += (int)gridDim.x * kEpiWarps) {
+        __nv_bfloat16* c = p.c + (long long)(i < front ? i : behind + i - front) * p.N;
         if (p.vec_out) {
           for (int n = lane * 8; n < p.N; n += 256) *reinterpret_cast<uint4*>(c + n) = make_uint4(0, 0, 0, 0);
         } else {

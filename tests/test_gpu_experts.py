@@ -990,3 +990,26 @@ def test_silu_mul_fp8_rows_whose_last_round_leaves_part_of_a_warp_idle(cols):
             values = _randn(rows, cols, dtype=dtype, seed=rows)
             q, scale = silu_mul_fp8(torch.cat([torch.full_like(values, 32.0), values], 1))
             _check_quotients(q, scale, values.float() * 32)
+
+
+@pytest.mark.parametrize("counts,lo,hi", [([40, 0, 30, 50], 1, 3), ([40, 0, 30, 50], 2, 4), ([700, 300, 5], 1, 2), ([3, 2, 90], 2, 3), ([0, 9], 0, 1)])
+def test_fp8_grouped_gemm_some_of_the_experts(counts, lo, hi):
+    """A slice of the experts and of their offsets: rows in front of the first and behind the last are zero, whatever the
+    memory held, and those of a given c stay."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import check, fp8_grouped_gemm
+
+    for n in (264, 129):
+        a, b, a_scale, b_scale, offsets = _grouped_inputs(counts, n, 256)
+        want = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+        first, last = offsets[lo].item(), offsets[hi].item()
+        own = torch.zeros(a.shape[0], dtype=torch.bool, device="cuda")
+        own[first:last] = True
+        stale = [torch.full_like(want, float("nan")) for _ in range(4)]
+        torch.cuda.synchronize()
+        del stale  # (its memory is handed out again)
+        out = fp8_grouped_gemm(a, b[lo:hi], a_scale, b_scale[lo:hi], offsets[lo:hi + 1])
+        check()
+        assert torch.equal(out[own], want[own]) and bool((out[~own] == 0).all())
+        given = torch.full_like(want, 7.0)
+        fp8_grouped_gemm(a, b[lo:hi], a_scale, b_scale[lo:hi], offsets[lo:hi + 1], c=given)
+        assert torch.equal(given[own], want[own]) and bool((given[~own] == 7).all())
