@@ -39,7 +39,8 @@ struct Fp8GroupedArgs {
   const void* b;          // [E, N, K] e4m3, row-major
   const float* a_scale;   // [M, ceil(K / 128)]
   const float* b_scale;   // [E, ceil(N / 128), ceil(K / 128)]
-  const int32_t* offsets; // [E + 1], device memory; cut off at 0 and M, and refused where they give more than M rows
+  const int32_t* offsets; // [E + 1], device memory; cut off at 0 and M, refused where they give more than M rows; one
+                          // below another in front of it counts as that
   void* c;                // [M, N] bf16 row-major
   int M, N, K, experts;
   long long as_stride_m, as_stride_k, bs_stride_e, bs_stride_n, bs_stride_k;  // element strides of the scale tensors

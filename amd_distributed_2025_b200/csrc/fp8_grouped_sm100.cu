@@ -76,6 +76,7 @@ static_assert(kNotes > kScaleSlots + 1, "a tile has a slot of scales at least: n
 constexpr int kMaxDynamicSmem = 232448 - 256;
 constexpr int kTmemCols = 512;
 constexpr int kBigBox = 64, kSmallBox = 16;  // rows of a copy of tokens
+constexpr long long kFall = 1ll << 42;  // added to the sum of rows (2^10 counts below 2^31) for an offset below the one before it
 
 struct GroupedParams {
   const float* a_scale;
@@ -221,20 +222,23 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   // The tables: a run of experts to a thread, then a prefix over threads.  Offsets that give more rows than there are would
-  // name tiles without end: nothing is computed then, and the record says so.
+  // name tiles without end: nothing is computed then, and the record says so.  Fewer rows, with offsets that fall, would give
+  // some of them to two experts, whose tiles would write them at the same time: an offset counts as the largest up to it
+  // then, which one thread works out.
   {
     const int each = (p.experts + kThreads - 1) / kThreads;
     const int lo = min(p.experts, tid * each), hi = min(p.experts, lo + each);
     int own = 0;
     long long rows = 0;
     for (int e = lo; e < hi; ++e) {
-      const int from = min(max(__ldcg(p.offsets + e), 0), p.M);
-      const int to = min(max(__ldcg(p.offsets + e + 1), from), p.M);
+      const int here = __ldcg(p.offsets + e), next = __ldcg(p.offsets + e + 1);
+      const int from = min(max(here, 0), p.M);
+      const int to = min(max(next, from), p.M);
       tables.start[e] = from;
       tables.count[e] = to - from;
       own += (to - from + kBt - 1) / kBt * p.n_tiles;
       tables.tiles_end[e] = own;
-      rows += to - from;
+      rows += to - from + (next < here ? kFall : 0);
     }
     int upto = own;
 #pragma unroll
@@ -251,8 +255,24 @@ fp8_grouped_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     for (int w = 0; w < warp; ++w) before += warp_sums[w];
     rows = 0;
     for (int w = 0; w < kThreads / 32; ++w) rows += warp_rows[w];
+    const bool falls = rows >= kFall;
+    rows %= kFall;
     const bool bad = rows > p.M;
     for (int e = lo; e < hi; ++e) tables.tiles_end[e] = bad ? 0 : tables.tiles_end[e] + before;
+    if (falls && !bad) {
+      __syncthreads();
+      if (tid == 0) {
+        int from = min(max(__ldcg(p.offsets), 0), p.M), tiles = 0;
+        for (int e = 0; e < p.experts; ++e) {
+          const int to = min(max(__ldcg(p.offsets + e + 1), from), p.M);
+          tables.start[e] = from;
+          tables.count[e] = to - from;
+          tiles += (to - from + kBt - 1) / kBt * p.n_tiles;
+          tables.tiles_end[e] = tiles;
+          from = to;
+        }
+      }
+    }
     if (bad && blockIdx.x == 0 && tid == 0 && p.status != nullptr)
       store_status(p.status, STATUS_BAD_INDEX, PHASE_NONE, -1, p.experts, 0, (uint64_t)rows);
   }

@@ -86,7 +86,8 @@ def fp8_grouped_gemm(
     or, in a ``c`` that is given, left as they were.
 
     Expired waits are reported as those of ``fp8_gemm`` are, by ``check()`` or the next call on the device, and so are
-    offsets that give the experts more rows than there are (nothing is computed then)."""
+    offsets that give the experts more rows than there are (nothing is computed then).  Where offsets fall and give no more,
+    one that is below another in front of it counts as that: no row has two experts."""
     ext = _ext.load()
     while True:
         out = ext.fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c, int(timeout_ms * 1e6))

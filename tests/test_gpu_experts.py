@@ -1013,3 +1013,30 @@ def test_fp8_grouped_gemm_some_of_the_experts(counts, lo, hi):
         given = torch.full_like(want, 7.0)
         fp8_grouped_gemm(a, b[lo:hi], a_scale, b_scale[lo:hi], offsets[lo:hi + 1], c=given)
         assert torch.equal(given[own], want[own]) and bool((given[~own] == 7).all())
+
+
+def test_fp8_grouped_gemm_offsets_that_fall_give_no_row_to_two_experts():
+    from amd_distributed_2025_b200.ops.fp8_gemm import check, fp8_grouped_gemm
+    from amd_distributed_2025_b200.utils.status import StatusError
+
+    for falling in ([10, 60, 20, 90, 80, 120], [0, 50, 40, 30, 20, 70], [0, 100, 90, 5, 60, 70], [-5, 40, 10, 5, 60, 300], [300, 0, 0, 0, 0, 0],
+                    [100, 90, 2 ** 31 - 1, -2 ** 31, 5, 290], [0] * 700 + [40, 20, 60, 1]):
+        experts = len(falling) - 1
+        for rows in (300, 5000) if experts < 100 else (300,):  # both kernels
+            a, b, a_scale, b_scale, _ = _grouped_inputs([rows] + [0] * (experts - 1), 136, 144)
+            offsets = torch.tensor(falling, dtype=torch.int32, device="cuda")
+            cut = [min(max(v, 0), rows) for v in falling]
+            if sum(max(there - here, 0) for here, there in zip(cut, cut[1:])) > rows:  # more rows than there are
+                fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+                with pytest.raises(StatusError, match="bad_index"):
+                    check()
+                continue
+            rising = offsets.clamp(0, rows).cummax(0).values.int()
+            got = fp8_grouped_gemm(a, b, a_scale, b_scale, offsets)
+            check()
+            assert torch.equal(got, fp8_grouped_gemm(a, b, a_scale, b_scale, rising))
+            _check_grouped((a, b, a_scale, b_scale, rising), got)
+            given = torch.full_like(got, 7.0)
+            fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c=given)
+            assert torch.equal(given[rising[0]:rising[-1]], got[rising[0]:rising[-1]])
+            assert bool((given[:rising[0]] == 7).all()) and bool((given[rising[-1]:] == 7).all())
