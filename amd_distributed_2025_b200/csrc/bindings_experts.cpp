@@ -213,6 +213,7 @@ PyObject* sort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
       TORCH_CHECK(scale_in->dim() == 2 && scale_in->size(0) == tokens && scale_in->size(1) >= 1 &&
                       scale_in->size(1) <= INT32_MAX / 8 && scale_in->scalar_type() == at::kFloat,
                   "scale must be float32 [tokens, scales of a row]");
+      check_no_gradient(*scale_in, "scale");
     }
     TORCH_CHECK(x_in.is_cuda(), "x must be a CUDA tensor");
     check_device(indices_in, x_in, "indices");
@@ -397,6 +398,11 @@ PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* v, Py_ssize_t n) {
       TORCH_CHECK(c->scalar_type() == at::kBFloat16 && c->dim() == 2 && c->size(0) == M && c->size(1) == N && c->is_contiguous(),
                   "c must be bf16 [M, N], row-major");
     TORCH_CHECK(timeout_ns > 0, "timeout_ms must be positive");
+    check_no_gradient(a_in, "a");
+    check_no_gradient(b_in, "b");
+    check_no_gradient(a_scale, "a_scale");
+    check_no_gradient(b_scale, "b_scale");
+    if (c) check_no_gradient(*c, "c");
     TORCH_CHECK(a_in.is_cuda(), "a must be a CUDA tensor");
     check_device(b_in, a_in, "b");
     check_device(a_scale, a_in, "a_scale");

@@ -83,7 +83,7 @@ def fp8_grouped_gemm(
     ``b_scale [E, ceil(N/128), ceil(K/128)]`` fp32 with any strides, ``offsets [E + 1]`` int32 on the device, not
     decreasing (``sort_tokens(...).order.offsets``, or a slice of them with the same experts of ``b``); experts may have no
     rows.  Returns bf16 ``[M, N]``.  Rows that no expert has, in front of ``offsets[0]`` and behind ``offsets[E]``, are zero,
-    or, in a ``c`` that is given, left as they were.
+    or, in a ``c`` that is given, left as they were.  There is no gradient; tensors that want one are refused.
 
     Expired waits are reported as those of ``fp8_gemm`` are, by ``check()`` or the next call on the device, and so are
     offsets that give the experts more rows than there are (nothing is computed then).  Where offsets fall and give no more,

@@ -52,7 +52,8 @@ def sort_tokens(
     """Copies row ``t`` of ``x [T, H]`` (fp16, bf16, fp32 or float8_e4m3fn) to a row for each of its experts
     ``indices [T, k]`` (int32 or int64, k <= 32, num_experts <= 8192), packed expert by expert.
 
-    ``scale [T, S]`` (fp32) goes the same way: the block scales of e4m3 rows."""
+    ``scale [T, S]`` (fp32) goes the same way: the block scales of e4m3 rows.  It has no gradient, and neither has ``x`` beside
+    it: what wants one is refused."""
     ext = _ext.load()
     got = ext.sort_tokens(x, indices, num_experts, scale)
     if got is None:  # x wants a gradient

@@ -142,3 +142,25 @@ def test_grouped_product_leaves_no_room_for_a_cta_that_waits_for_tensor_memory()
     for smem, columns in own:
         assert columns == 512 and smem <= 232448
         assert smem + reserved + min(others + [s for s, _ in own]) + reserved > sm
+
+
+def test_scales_that_want_a_gradient_are_refused():
+    """Neither operator has one: e4m3 rows cannot have a gradient themselves, but their scales can want one."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+
+    fp8 = torch.float8_e4m3fn
+    ids = F(4, 2, dtype=torch.int32)
+    for x in (F(4, 256).to(fp8), F(4, 256)):
+        _refused("scale requires a gradient", lambda: moe_sort.sort_tokens(x, ids, 8, scale=F(4, 2).requires_grad_()))
+        _refused("scale requires a gradient", lambda: moe_sort.sort_tokens(x, ids, 8, scale=F(4, 2).requires_grad_() * 2))
+        with torch.no_grad():
+            _refused("CUDA", lambda: moe_sort.sort_tokens(x, ids, 8, scale=F(4, 2).requires_grad_()))
+    off = F(4, dtype=torch.int32)
+    names = ("a", "b", "a_scale", "b_scale", "c")
+    for i, name in enumerate(names):
+        given = [F(4, 256).to(fp8), F(3, 130, 256).to(fp8), F(4, 2), F(3, 2, 2), F(4, 130, dtype=torch.bfloat16)]
+        given[i].requires_grad_()
+        a, b, a_scale, b_scale, c = given
+        _refused(f"^{name} requires a gradient", lambda: fp8_grouped_gemm(a, b, a_scale, b_scale, off, c))
+        with torch.no_grad():
+            _refused("CUDA", lambda: fp8_grouped_gemm(a, b, a_scale, b_scale, off, c))
