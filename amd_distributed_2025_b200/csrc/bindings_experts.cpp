@@ -55,14 +55,19 @@ at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Tensor
   return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
 }
 
-// ------------------------------------------------------------- rows with block scales ----
-
 bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
+// (a result without a tangent would count as one whose tangent is zero)
+void check_no_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), what, " has a forward-mode tangent, and this operator has no forward derivative");
+}
 void check_no_gradient(const at::Tensor& t, const char* what) {
+  check_no_tangent(t, what);
   TORCH_CHECK(!wants_gradient(t), what,
               " requires a gradient, and this operator has none: call it under torch.no_grad()");
 }
+
+// ------------------------------------------------------------- rows with block scales ----
 
 // Two matrices of one shape and type, of which one is written while the other is read: the very same rows are fine (a lane
 // reads its columns before it writes them), and so are rows that do not meet.
@@ -195,6 +200,7 @@ PyObject* sort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     count_args(n, 4);
     const at::Tensor& x_in = tensor_arg(v[0]);
+    check_no_tangent(x_in, "x");
     if (wants_gradient(x_in)) Py_RETURN_NONE;
     const at::Tensor& indices_in = tensor_arg(v[1]);
     const int64_t experts = int_arg(v[2]);
@@ -270,6 +276,8 @@ PyObject* unsort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const at::Tensor& rows_in = tensor_arg(v[0]);
     const at::Tensor& row_of_in = tensor_arg(v[1]);
     const optional<at::Tensor> weights_in = optional_arg(v[2]);
+    check_no_tangent(rows_in, "rows");
+    if (weights_in) check_no_tangent(*weights_in, "weights");
     if (wants_gradient(rows_in) || (weights_in && (wants_gradient(*weights_in) || weights_in->scalar_type() != at::kFloat)))
       Py_RETURN_NONE;
     TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(1) >= 1 && rows_in.size(1) <= INT32_MAX / 8, "rows must be a matrix [rows, hidden]");
@@ -325,6 +333,9 @@ PyObject* unsort_tokens_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
     TORCH_CHECK(grad_in.dim() == 2 && grad_in.size(0) == tokens && grad_in.size(1) == hidden && grad_in.scalar_type() == type,
                 "the gradient must be [tokens, hidden] of the rows' type");
     if (weights_in) weights_of(*weights_in, row_of_in);
+    check_no_tangent(grad_in, "the gradient");
+    check_no_tangent(rows_in, "rows");
+    if (weights_in) check_no_tangent(*weights_in, "weights");
     TORCH_CHECK(rows_in.is_cuda(), "rows must be a CUDA tensor");
     check_device(grad_in, rows_in, "the gradient");
     check_device(offsets_in, rows_in, "offsets");

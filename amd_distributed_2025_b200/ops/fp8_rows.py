@@ -11,8 +11,8 @@ Of a block of 128 columns (the last one of a row may be shorter) ``scale = max(m
 All of it is fp32 between the loads and the one rounding of each output (csrc/fp8_rows.cu).
 
 Inputs are CUDA matrices in fp16, bf16 or fp32 (all of a call of one type; the weight may be fp32 beside the others),
-with any distance between rows; rows that are not contiguous are copied first.  The operators have no gradient and
-refuse inputs that want one.  They launch on the current stream of the inputs' device.
+with any distance between rows; rows that are not contiguous are copied first.  The operators have no gradient, in
+neither mode, and refuse inputs that want one.  They launch on the current stream of the inputs' device.
 """
 from __future__ import annotations
 

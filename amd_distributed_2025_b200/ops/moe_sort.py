@@ -13,7 +13,7 @@ Inside an expert rows are in (token, k) order, as in the dispatch layout.  An en
 expert's are zero, in gradients too.  A token may name an expert twice and has two rows then.  Sums are fp32, over k
 upwards, rounded once; nothing depends on an order of atomics.
 
-Both are differentiable (fp16, bf16, fp32).  The gradients can be had without autograd too:
+Both are differentiable (fp16, bf16, fp32) in reverse mode; forward-mode tangents are refused.  The gradients can be had without autograd too:
 ``sort_tokens_backward`` and ``unsort_tokens_backward``.  All of it may be captured into a CUDA graph; a forward pass that
 is captured while an eager graph of the same leaves is alive is refused (their gradients are added up on the eager
 graph's stream, for which a captured backward pass cannot wait).
@@ -98,10 +98,11 @@ def unsort_tokens_backward(
 
 
 def _refuse_foreign_leaves(ext, *tensors: Optional[torch.Tensor]) -> None:
-    if not torch.cuda.is_current_stream_capturing():
+    on_gpu = [t for t in tensors if t is not None and t.is_cuda]
+    if not on_gpu or not torch.cuda.is_current_stream_capturing():
         return
-    for t in tensors:
-        if t is not None and t.is_cuda and ext.adds_up_elsewhere(t):
+    for t in on_gpu:
+        if ext.adds_up_elsewhere(t):
             raise RuntimeError("a backward pass cannot be captured while an eager graph of the same leaves is alive: "
                                "drop that graph (its outputs and losses) before the capture")
 

@@ -164,3 +164,46 @@ def test_scales_that_want_a_gradient_are_refused():
         _refused(f"^{name} requires a gradient", lambda: fp8_grouped_gemm(a, b, a_scale, b_scale, off, c))
         with torch.no_grad():
             _refused("CUDA", lambda: fp8_grouped_gemm(a, b, a_scale, b_scale, off, c))
+
+
+def test_forward_mode_tangents_are_refused():
+    """No operator here has a forward derivative, and a result without a tangent would count as one of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+
+    fp8 = torch.float8_e4m3fn
+    ids, off = F(4, 2, dtype=torch.int32), F(4, dtype=torch.int32)
+    order = ExpertOrder(F(9, dtype=torch.int32), ids)
+    x, w, rows, routing = F(4, 256), F(256), F(8, 64), F(4, 2)
+    a, b, sa, sb = F(4, 256).to(fp8), F(3, 130, 256).to(fp8), F(4, 2), F(3, 2, 2)
+    with fwd.dual_level():
+        def d(t, grad=False):
+            return fwd.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+
+        calls = [
+            ("x", lambda: fp8_rows.rms_norm_fp8(d(x), w)),
+            ("weight", lambda: fp8_rows.rms_norm_fp8(x, d(w))),
+            ("residual", lambda: fp8_rows.rms_norm_fp8(x, w, residual=d(x))),
+            ("total_out", lambda: fp8_rows.rms_norm_fp8(x, w, residual=x, total_out=d(x))),
+            ("x", lambda: fp8_rows.silu_mul_fp8(d(x))),
+            ("x", lambda: moe_sort.sort_tokens(d(x), ids, 8)),
+            ("x", lambda: moe_sort.sort_tokens(d(x, True), ids, 8)),
+            ("scale", lambda: moe_sort.sort_tokens(x, ids, 8, scale=d(F(4, 2)))),
+            ("rows", lambda: moe_sort.unsort_tokens(d(rows), order, routing)),
+            ("weights", lambda: moe_sort.unsort_tokens(rows, order, d(routing))),
+            ("weights", lambda: moe_sort.unsort_tokens(rows, order, d(routing.half()))),
+            ("rows", lambda: moe_sort.unsort_tokens(d(rows, True), order, routing)),
+            ("the gradient", lambda: moe_sort.unsort_tokens_backward(d(F(4, 64)), rows, order, routing)),
+            ("rows", lambda: moe_sort.unsort_tokens_backward(F(4, 64), d(rows), order, routing)),
+            ("weights", lambda: moe_sort.unsort_tokens_backward(F(4, 64), rows, order, d(routing))),
+            ("rows", lambda: moe_sort.sort_tokens_backward(d(rows), order)),
+            ("a_scale", lambda: fp8_grouped_gemm(a, b, d(sa), sb, off)),
+            ("b_scale", lambda: fp8_grouped_gemm(a, b, sa, d(sb), off)),
+            ("c", lambda: fp8_grouped_gemm(a, b, sa, sb, off, d(F(4, 130, dtype=torch.bfloat16)))),
+        ]
+        for name, call in calls:
+            _refused(f"^{name} has a forward-mode tangent", call)
+            with torch.no_grad():
+                _refused(f"^{name} has a forward-mode tangent", call)
+    _refused("CUDA", lambda: moe_sort.sort_tokens(x, ids, 8))
