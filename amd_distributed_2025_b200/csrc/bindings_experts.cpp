@@ -51,6 +51,11 @@ void check_device(const at::Tensor& t, const at::Tensor& first, const char* what
 at::Tensor with_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
+// A caller's tensor has been written: what autograd has saved of it before is no longer what it was.
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
   return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
 }
@@ -125,6 +130,7 @@ PyObject* rms_norm_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {
       at::assert_no_overlap(*total, weight_in);
     }
     c10::cuda::CUDAGuard guard(x_in.device());
+    if (total) changed(*total);
     const at::Tensor x = with_rows(x_in), weight = weight_in.contiguous();
     at::Tensor residual;
     if (residual_in) {
@@ -426,7 +432,8 @@ PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     c10::cuda::CUDAGuard guard(a_in.device());
     if (fp8_status_code(a_in.get_device()) != 0) Py_RETURN_NONE;
     const bool zero_rest = !c;
-    if (!c) c = new_cuda({M, N}, at::kBFloat16, a_in);
+    if (c) changed(*c);
+    else c = new_cuda({M, N}, at::kBFloat16, a_in);
     if (M == 0) return wrap(c);
     const at::Tensor a = for_copies(a_in), b = for_copies(b_in), offsets = offsets_in.contiguous();
     b200::Fp8GroupedArgs g = {};

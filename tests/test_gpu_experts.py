@@ -1040,3 +1040,37 @@ def test_fp8_grouped_gemm_offsets_that_fall_give_no_row_to_two_experts():
             fp8_grouped_gemm(a, b, a_scale, b_scale, offsets, c=given)
             assert torch.equal(given[rising[0]:rising[-1]], got[rising[0]:rising[-1]])
             assert bool((given[:rising[0]] == 7).all()) and bool((given[rising[-1]:] == 7).all())
+
+
+def test_outputs_in_place_count_as_changes():
+    """What autograd has saved and total_out or c then overwrites is noticed by the backward pass, as with torch's own operations."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    x, w = _randn(4, 256, seed=1), _randn(256, seed=2)
+    inputs = _grouped_inputs([3, 5], 256, 128)
+
+    def saved(values):
+        scale = torch.ones(256, device="cuda", requires_grad=True)
+        return (scale * values).sum()
+
+    residual = _randn(4, 256, seed=3)
+    c = torch.ones(8, 256, dtype=torch.bfloat16, device="cuda")
+    for target, write in ((residual, lambda: rms_norm_fp8(x, w, residual=residual, total_out=residual)),
+                          (x, lambda: rms_norm_fp8(x, w, residual=residual, total_out=x)),
+                          (residual, lambda: rms_norm_fp8(x[:2], w, residual=x[2:], total_out=residual[1:3])),  # a view
+                          (c, lambda: fp8_grouped_gemm(*inputs, c=c))):
+        loss = saved(target)
+        with torch.no_grad():
+            write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        saved(target).backward()
+    loss = saved(x)  # nothing of it is written
+    fresh = rms_norm_fp8(x, w, residual=residual)
+    loss.backward()
+    with torch.inference_mode():  # (tensors that count no changes)
+        out = torch.empty(4, 256, device="cuda")
+        assert torch.equal(rms_norm_fp8(x, w, residual=residual, total_out=out).total, fresh.total)
+        inside = torch.empty_like(c)
+        assert torch.equal(fp8_grouped_gemm(*inputs, c=inside), c)
