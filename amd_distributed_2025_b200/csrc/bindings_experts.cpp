@@ -317,44 +317,47 @@ PyObject* unsort_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// (grad, rows, offsets, row_of, weights or None, want_rows, want_weights) -> (grad_rows or None, grad_weights or None)
+// (grad, rows, offsets, row_of, weights or None, want_rows, want_weights) -> (grad_rows or None, grad_weights or None); rows
+// may be None where the weights' gradient is not wanted
 PyObject* unsort_tokens_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&] {
     count_args(n, 7);
     const at::Tensor& grad_in = tensor_arg(v[0]);
-    const at::Tensor& rows_in = tensor_arg(v[1]);
+    const optional<at::Tensor> rows_in = optional_arg(v[1]);
     const at::Tensor& offsets_in = tensor_arg(v[2]);
     const at::Tensor& row_of_in = tensor_arg(v[3]);
     const optional<at::Tensor> weights_in = optional_arg(v[4]);
     const bool want_rows = bool_arg(v[5]), want_weights = bool_arg(v[6]) && weights_in;
-    const auto type = rows_in.scalar_type();
+    const at::Tensor& like = rows_in ? *rows_in : grad_in;
+    const auto type = like.scalar_type();
     const int code = dtype_code(type);
     check_order(row_of_in, "row_of");
     TORCH_CHECK(offsets_in.dim() == 1 && offsets_in.size(0) >= 2 && offsets_in.scalar_type() == at::kInt, "offsets must be int32 [num_experts + 1]");
     const int64_t tokens = row_of_in.size(0), k = row_of_in.size(1);
-    TORCH_CHECK(rows_in.dim() == 2 && rows_in.size(1) >= 1 && rows_in.size(1) <= INT32_MAX / 8 &&
-                    rows_in.size(0) == check_entries(tokens, k),
-                "rows must have a row for each of the ", num(tokens * k), " entries");
-    const int64_t hidden = rows_in.size(1), entries = tokens * k;
+    const int64_t entries = check_entries(tokens, k);
+    TORCH_CHECK(like.dim() == 2 && like.size(1) >= 1 && like.size(1) <= INT32_MAX / 8 && (!rows_in || rows_in->size(0) == entries),
+                "rows must have a row for each of the ", num(entries), " entries");
+    TORCH_CHECK(rows_in || !want_weights, "the weights' gradient needs the rows");
+    const int64_t hidden = like.size(1);
     TORCH_CHECK(grad_in.dim() == 2 && grad_in.size(0) == tokens && grad_in.size(1) == hidden && grad_in.scalar_type() == type,
                 "the gradient must be [tokens, hidden] of the rows' type");
     if (weights_in) weights_of(*weights_in, row_of_in);
     check_no_tangent(grad_in, "the gradient");
-    check_no_tangent(rows_in, "rows");
+    if (rows_in) check_no_tangent(*rows_in, "rows");
     if (weights_in) check_no_tangent(*weights_in, "weights");
-    TORCH_CHECK(rows_in.is_cuda(), "rows must be a CUDA tensor");
-    check_device(grad_in, rows_in, "the gradient");
-    check_device(offsets_in, rows_in, "offsets");
-    check_device(row_of_in, rows_in, "row_of");
-    if (weights_in) check_device(*weights_in, rows_in, "weights");
-    c10::cuda::CUDAGuard guard(rows_in.device());
+    TORCH_CHECK(like.is_cuda(), rows_in ? "rows" : "the gradient", " must be a CUDA tensor");
+    check_device(grad_in, like, "the gradient");
+    check_device(offsets_in, like, "offsets");
+    check_device(row_of_in, like, "row_of");
+    if (weights_in) check_device(*weights_in, like, "weights");
+    c10::cuda::CUDAGuard guard(like.device());
     optional<at::Tensor> grad_rows, grad_weights;
-    if (want_rows) grad_rows = new_cuda({entries, hidden}, type, rows_in);
-    if (want_weights) grad_weights = new_cuda({tokens, k}, at::kFloat, rows_in);
+    if (want_rows) grad_rows = new_cuda({entries, hidden}, type, like);
+    if (want_weights) grad_weights = new_cuda({tokens, k}, at::kFloat, like);
     if (!want_rows && !want_weights) return tuple_of({grad_rows, grad_weights});
     const at::Tensor grad = with_rows(grad_in), offsets = offsets_in.contiguous(), row_of = row_of_in.contiguous();
     at::Tensor rows, weights;
-    if (want_weights) rows = with_rows(rows_in);
+    if (want_weights) rows = with_rows(*rows_in);
     if (weights_in) weights = weights_in->contiguous();
     b200::UnsortBackwardArgs a = {};
     a.grad = grad.const_data_ptr();
@@ -371,7 +374,7 @@ PyObject* unsort_tokens_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
     a.k = (int32_t)k;
     a.hidden = (int32_t)hidden;
     a.dtype = code;
-    cuda_check(b200::launch_unsort_tokens_backward(a, device_sms(rows_in.get_device()), at::cuda::getCurrentCUDAStream()),
+    cuda_check(b200::launch_unsort_tokens_backward(a, device_sms(like.get_device()), at::cuda::getCurrentCUDAStream()),
                "unsort_tokens_backward launch");
     return tuple_of({grad_rows, grad_weights});
   });

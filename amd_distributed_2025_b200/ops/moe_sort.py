@@ -127,7 +127,7 @@ class _Sort(torch.autograd.Function):
 class _Unsort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, offsets, row_of, weights):
-        ctx.save_for_backward(rows, offsets, row_of, weights)
+        ctx.save_for_backward(rows if ctx.needs_input_grad[3] else None, offsets, row_of, weights)
         return _ext.load().unsort_tokens(rows, row_of, weights)
 
     @staticmethod

@@ -1074,3 +1074,41 @@ def test_outputs_in_place_count_as_changes():
         assert torch.equal(rms_norm_fp8(x, w, residual=residual, total_out=out).total, fresh.total)
         inside = torch.empty_like(c)
         assert torch.equal(fp8_grouped_gemm(*inputs, c=inside), c)
+
+
+def test_unsort_keeps_rows_for_the_weights_gradient_only():
+    """The rows' own gradient does not need them: they are free to go when the weights want none."""
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    ids = _ids(40, 3, 8, 1, "skewed")
+    order = moe_sort.ExpertOrder(*_order_of(ids, 8))
+    grad = _randn(40, 72, seed=3)
+    routing = torch.rand(40, 3, device="cuda", generator=_gen(2))
+    for dtype in DTYPES:
+        leaf = _randn(120, 72, dtype=dtype, seed=1).requires_grad_()
+        for weights in (None, routing, routing.half(), routing.clone().requires_grad_()):
+            kept = []
+
+            def pack(t):
+                kept.append(t.data_ptr())
+                return t
+
+            rows = leaf * 1
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+                out = moe_sort.unsort_tokens(rows, order, weights)
+            wanted = weights is not None and weights.requires_grad
+            assert (rows.data_ptr() in kept) == wanted
+            out.backward(grad.to(dtype))
+            w32 = None if weights is None else weights.detach().float()
+            want = moe_sort.unsort_tokens_backward(grad.to(dtype), rows.detach(), order, w32)
+            assert torch.equal(leaf.grad, want[0])
+            if wanted:
+                assert torch.equal(weights.grad, want[1])
+            leaf.grad = None
+        only = routing.clone().requires_grad_()  # and the weights alone
+        moe_sort.unsort_tokens(leaf.detach(), order, only).backward(grad.to(dtype))
+        assert torch.equal(only.grad, moe_sort.unsort_tokens_backward(grad.to(dtype), leaf.detach(), order, routing)[1])
+    none = moe_sort.ExpertOrder(torch.zeros(9, dtype=torch.int32, device="cuda"), order.row_of[:0])
+    empty = torch.empty(0, 72, device="cuda", requires_grad=True)
+    moe_sort.unsort_tokens(empty, none).sum().backward()
+    assert empty.grad.shape == (0, 72)
