@@ -78,6 +78,9 @@ def unsort_tokens(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torc
         if not weights.dtype.is_floating_point:
             raise ValueError(f"weights must be of a floating type, not {weights.dtype}")
         weights = weights.to(torch.float32)
+        out = ext.unsort_tokens(rows, order.row_of, weights)
+        if out is not None:  # nothing wants a gradient
+            return out
     _refuse_foreign_leaves(ext, rows, weights)
     return _Unsort.apply(rows, order.offsets, order.row_of, weights)
 

@@ -1112,3 +1112,32 @@ def test_unsort_keeps_rows_for_the_weights_gradient_only():
     empty = torch.empty(0, 72, device="cuda", requires_grad=True)
     moe_sort.unsort_tokens(empty, none).sum().backward()
     assert empty.grad.shape == (0, 72)
+
+
+def test_unsort_without_gradient_is_captured_whatever_the_weights_type():
+    """No backward pass follows, so an eager graph of the rows and weights is no reason to refuse."""
+    from amd_distributed_2025_b200.ops import moe_sort
+
+    ids = _ids(16, 2, 4, 2)
+    order = moe_sort.ExpertOrder(*_order_of(ids, 4))
+    rows = _randn(32, 64, seed=1).requires_grad_()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16, torch.float64):
+        weights = torch.rand(16, 2, device="cuda", generator=_gen(3)).to(dtype).requires_grad_()
+        alive = (weights * 2).sum() + rows.sum()
+        with torch.no_grad():
+            want = moe_sort.unsort_tokens(rows, order, weights)
+            assert not want.requires_grad
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = moe_sort.unsort_tokens(rows, order, weights)
+        graph.replay()
+        assert torch.equal(got, want) and torch.equal(want, moe_sort.unsort_tokens(rows.detach(), order, weights.detach().float()))
+        refused = []
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):  # with a gradient it is still refused
+            try:
+                moe_sort.unsort_tokens(rows, order, weights)
+            except RuntimeError as e:
+                refused.append(str(e))
+        assert len(refused) == 1 and "eager graph" in refused[0]
+        del alive
