@@ -2,11 +2,11 @@
 // (moe_sort.h), the experts' fp8 products (fp8_gemm.h).  Shapes and types are looked at before devices, so that a wrong call is refused without a GPU too.
 #include "bindings_experts.h"
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <algorithm>
 #include <unordered_set>
 
 #include "bindings_common.h"
@@ -74,19 +74,35 @@ void check_no_gradient(const at::Tensor& t, const char* what) {
 
 // ------------------------------------------------------------- rows with block scales ----
 
+// Bytes from a tensor's first element to behind its last one.
+int64_t reach(const at::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return (last + 1) * (int64_t)t.element_size();
+}
+// Whether two tensors cannot share memory: one ends before the other begins, or both are columns of the same wider matrix (a
+// vector, or a matrix of one row, lies in one row of it).
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const int64_t between = (int64_t)((intptr_t)b.const_data_ptr() - (intptr_t)a.const_data_ptr());
+  if (between >= reach(a) || -between >= reach(b)) return true;
+  const auto width = [](const at::Tensor& t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? 0 : t.size(-1) * (int64_t)t.element_size(); };
+  const auto step = [](const at::Tensor& t) { return t.dim() == 2 && t.size(0) > 1 ? t.stride(0) * (int64_t)t.element_size() : 0; };
+  if (a.dim() < 1 || a.dim() > 2 || b.dim() < 1 || b.dim() > 2 || width(a) == 0 || width(b) == 0) return false;
+  const int64_t rows = std::max(step(a), step(b));
+  if (rows == 0 || (step(a) != rows && step(a) != 0) || (step(b) != rows && step(b) != 0)) return false;
+  const int64_t within = (between % rows + rows) % rows;
+  return within >= width(a) && within + width(b) <= rows;
+}
+void check_apart(const at::Tensor& a, const at::Tensor& b, const char* what) {
+  TORCH_CHECK(apart(a, b), what, " overlap in memory");
+}
 // Two matrices of one shape and type, of which one is written while the other is read: the very same rows are fine (a lane
-// reads its columns before it writes them), and so are rows that do not meet.
+// reads its columns before it writes them).
 void check_apart_or_same(const at::Tensor& a, const at::Tensor& b, const char* what) {
-  if (a.numel() == 0 || (a.const_data_ptr() == b.const_data_ptr() && a.strides() == b.strides())) return;
-  const int64_t bytes = (int64_t)a.element_size(), rows = a.size(0), cols = a.size(1);
-  const auto reach = [&](const at::Tensor& t) { return ((rows - 1) * t.stride(0) + (cols - 1) * t.stride(1) + 1) * bytes; };
-  const int64_t apart = (int64_t)((intptr_t)a.const_data_ptr() - (intptr_t)b.const_data_ptr());
-  if (apart >= reach(b) || -apart >= reach(a)) return;
-  if (a.strides() == b.strides() && (cols == 1 || a.stride(1) == 1)) {  // columns of the same wider matrix
-    const int64_t step = a.stride(0) * bytes, within = ((apart % step) + step) % step;
-    if (within >= cols * bytes && within <= step - cols * bytes) return;
-  }
-  TORCH_CHECK(false, what, " overlap in memory and are not the same");
+  const bool same = a.const_data_ptr() == b.const_data_ptr() && (a.size(0) <= 1 || a.stride(0) == b.stride(0)) &&
+                    (a.size(1) <= 1 || a.stride(1) == b.stride(1));
+  TORCH_CHECK(same || apart(a, b), what, " overlap in memory and are not the same");
 }
 
 // (x, weight, eps, residual or None, total_out or None, normed) -> (q, scale, total or None, normed or None)
@@ -119,16 +135,14 @@ PyObject* rms_norm_fp8(PyObject*, PyObject* const* v, Py_ssize_t n) {
       TORCH_CHECK((cols == 1 || total->stride(1) == 1) && (rows <= 1 || total->stride(0) >= cols),
                   "total_out must have contiguous rows that do not overlap");
       check_no_gradient(*total, "total_out");
+      check_apart_or_same(*total, x_in, "total_out and x");
+      check_apart_or_same(*total, *residual_in, "total_out and residual");
+      check_apart(*total, weight_in, "total_out and weight");
     }
     TORCH_CHECK(x_in.is_cuda(), "x must be a CUDA tensor");
     check_device(weight_in, x_in, "weight");
     if (residual_in) check_device(*residual_in, x_in, "residual");
-    if (total) {
-      check_device(*total, x_in, "total_out");
-      check_apart_or_same(*total, x_in, "total_out and x");
-      check_apart_or_same(*total, *residual_in, "total_out and residual");
-      at::assert_no_overlap(*total, weight_in);
-    }
+    if (total) check_device(*total, x_in, "total_out");
     c10::cuda::CUDAGuard guard(x_in.device());
     if (total) changed(*total);
     const at::Tensor x = with_rows(x_in), weight = weight_in.contiguous();
@@ -422,16 +436,20 @@ PyObject* fp8_grouped_gemm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     check_no_gradient(b_in, "b");
     check_no_gradient(a_scale, "a_scale");
     check_no_gradient(b_scale, "b_scale");
-    if (c) check_no_gradient(*c, "c");
+    if (c) {
+      check_no_gradient(*c, "c");
+      check_apart(*c, a_in, "c and a");
+      check_apart(*c, b_in, "c and b");
+      check_apart(*c, a_scale, "c and a_scale");
+      check_apart(*c, b_scale, "c and b_scale");
+      check_apart(*c, offsets_in, "c and offsets");
+    }
     TORCH_CHECK(a_in.is_cuda(), "a must be a CUDA tensor");
     check_device(b_in, a_in, "b");
     check_device(a_scale, a_in, "a_scale");
     check_device(b_scale, a_in, "b_scale");
     check_device(offsets_in, a_in, "offsets");
-    if (c) {
-      check_device(*c, a_in, "c");
-      for (const at::Tensor* t : {&a_in, &b_in, &a_scale, &b_scale, &offsets_in}) at::assert_no_overlap(*c, *t);
-    }
+    if (c) check_device(*c, a_in, "c");
     c10::cuda::CUDAGuard guard(a_in.device());
     if (fp8_status_code(a_in.get_device()) != 0) Py_RETURN_NONE;
     const bool zero_rest = !c;

@@ -207,3 +207,53 @@ def test_forward_mode_tangents_are_refused():
             with torch.no_grad():
                 _refused(f"^{name} has a forward-mode tangent", call)
     _refused("CUDA", lambda: moe_sort.sort_tokens(x, ids, 8))
+
+
+def test_outputs_that_share_memory_with_inputs():
+    """Refused unless they are the very same rows, or columns of one wider matrix that do not meet."""
+    from amd_distributed_2025_b200.ops.fp8_gemm import fp8_grouped_gemm
+
+    w = F(8)
+    f = fp8_rows.rms_norm_fp8
+
+    def norm(x, residual, total, weight=w):
+        return lambda: f(x, weight, residual=residual, total_out=total)
+
+    flat = F(1000)
+    # one row, whatever the distance to a next one says (0 divides nothing)
+    for one, other in ((0, 0), (8, 0), (0, 8), (8, 100), (3, 5)):
+        x, total = flat.as_strided((1, 8), (one, 1), 4), flat.as_strided((1, 8), (other, 1), 0)
+        _refused("total_out and x overlap", norm(x, F(1, 8), total))
+        _refused("total_out and residual overlap", norm(F(1, 8), x, total))
+        same = flat.as_strided((1, 8), (one, 1), 0)
+        _refused("CUDA", norm(same, F(1, 8), total))
+        _refused("CUDA", norm(F(1, 8), same, total))
+        _refused("CUDA", norm(flat.as_strided((1, 8), (one, 1), 8), F(1, 8), total))
+    wide = flat.view(20, 50)
+    total = wide[:, 10:18]
+    for lo, fine in ((0, True), (2, True), (3, False), (10, True), (17, False), (18, True), (42, True)):
+        _refused("CUDA" if fine else "overlap", norm(wide[:, lo:lo + 8], F(20, 8), total))
+        _refused("CUDA" if fine else "overlap", norm(F(20, 8), wide[:, lo:lo + 8], total))
+    _refused("overlap", norm(wide[:1, 10:18].expand(20, 8), F(20, 8), total))  # one row of it, read again and again
+    _refused("CUDA", norm(wide[:1, 20:28].expand(20, 8), F(20, 8), total))
+    _refused("overlap", norm(flat[4:164].view(20, 8), F(20, 8), total))
+    # the weight in the sum's rows, and between them
+    _refused("total_out and weight overlap", norm(F(20, 8), F(20, 8), total, wide[3, 10:18]))
+    _refused("total_out and weight overlap", norm(F(20, 8), F(20, 8), total, wide[3, 4:12]))
+    _refused("total_out and weight overlap", norm(F(20, 8), F(20, 8), total, wide[:8, 10]))
+    _refused("CUDA", norm(F(20, 8), F(20, 8), total, wide[3, 20:28]))
+    _refused("CUDA", norm(F(20, 8), F(20, 8), total, flat[:8]))
+    _refused("CUDA", norm(F(0, 8), F(0, 8), wide[:0, :8]))
+    # a product's result and inputs whose strides leave room in between
+    fp8 = torch.float8_e4m3fn
+    a, b, sb, off = F(4, 256).to(fp8), F(3, 130, 256).to(fp8), F(3, 2, 2), F(4, dtype=torch.int32)
+    room = F(4000)
+    c = room[:260].view(torch.bfloat16).view(4, 130)
+    _refused("c and a_scale overlap", lambda: fp8_grouped_gemm(a, b, room.as_strided((4, 2), (100, 2), 10), sb, off, c))
+    _refused("c and b_scale overlap", lambda: fp8_grouped_gemm(a, b, F(4, 2), room.as_strided((3, 2, 2), (1000, 100, 10), 9), off, c))
+    _refused("c and a overlap", lambda: fp8_grouped_gemm(room.view(fp8).view(4, 4000)[:, :256], b, F(4, 2), sb, off, c))
+    raw = F(25000)
+    inside = raw[10:270].view(torch.bfloat16).view(4, 130)
+    _refused("c and b overlap", lambda: fp8_grouped_gemm(a, raw.view(fp8)[:99840].view(3, 130, 256), F(4, 2), sb, off, inside))
+    _refused("c and offsets overlap", lambda: fp8_grouped_gemm(a, b, F(4, 2), sb, room[255:259].view(torch.int32), c))
+    _refused("CUDA", lambda: fp8_grouped_gemm(a, b, room.as_strided((4, 2), (100, 2), 260), sb, room[800:804].view(torch.int32), c))
