@@ -17,10 +17,10 @@
 // fp32 registers while the other is being filled.  Pairs are persistent, and walk the same list of tiles: experts in order,
 // an expert's in bands, so that pairs at work at the same time share weights and tokens in L2.
 //
-// What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 535 us, 7.0
-// TB/s in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x 4096, one expert: 122 us,
-// 121 there, 2.25 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights) is between the two:
-// 478 us at first, 535 to 570 where calls follow on one another for a second: power, at 1.3 to 1.4 GHz.
+// What bounds it: few rows, the weights out of memory (256 experts of 2048 x 7168 with 4 rows each: 3.76 GB in 525 to 568 us
+// from box to box, 6.6 to 7.2 TB/s, in a row of calls); many rows, the chain of an epilogue warp, as in fp8_gemm (8192 x 4096 x
+// 4096, one expert: 122 us, 121 there, 2.25 PFLOP/s); skewed routing (24576 rows over 64 experts of 4096 x 4096, 1 GB of weights)
+// is between the two: 478 us at first, 535 to 584 where calls follow on one another for a second: power, at 1.3 to 1.4 GHz.
 // What it took, us at 8192 rows of one expert / of 64 experts / at 256 experts with 4 rows each:
 //   tokens always on the free side, up to 256 of them, 16 x 256 bits           154 / 232 / 570
 //   the next piece out of tensor memory while one is added up                  176 / 208 / 552   (registers spill)

@@ -80,8 +80,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// g / (1 + exp(-g)) * u of two values, with the sign changed.  A gate below -87.3 has a sum above 2^126 and counts beside values
-// near 1e36: a quarter of the sum still has a reciprocal that is a normal number.  (An exponential that is none adds nothing to 1.)
+// g / (1 + exp(-g)) * u of two values, with the sign changed.  A gate below -87.3 has a sum above 2^126 and counts beside
+// values near 1e36: a quarter of the sum still has a reciprocal that is a normal number.  (An exponential that is none adds
+// nothing to 1.)
 __device__ __forceinline__ float2 minus_silu_mul(float2 g, float2 u) {
   const float2 x = mul2(g, make_float2(-1.44269504f, -1.44269504f));  // log2(e)
   float2 e;
@@ -207,8 +208,8 @@ struct Lanes {
         if (c + 32 * e < cols) row[c + 32 * e] = from_f32<T>(f[e]);
     }
   }
-  // Block scale and e4m3 values of one unit (every lane of the warp takes part; columns behind the row hold zeros).  It is given
-  // -y: with q = -y * -1 / scale, y's remainder is -(q * scale + -y), and zeros keep their signs through all of it.
+  // Block scale and e4m3 values of one unit (every lane of the warp takes part; columns behind the row hold zeros).  It is
+  // given -y: with q = -y * -1 / scale, y's remainder is -(q * scale + -y), and zeros keep their signs through all of it.
   static __device__ __forceinline__ void quantise(uint8_t* q_row, float* scale_row, int u, int cols, const float* minus_y) {
     float most = fabsf(minus_y[0]);
 #pragma unroll
@@ -220,7 +221,7 @@ struct Lanes {
       for (int o = kUnits / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
     most = max_nan(most, kLeastMax);
-    const float scale = most * (1.f / kE4m3Max), inverse = -reciprocal(scale);  // (normal numbers both: 1e-30 is the least maximum)
+    const float scale = most * (1.f / kE4m3Max), inverse = -reciprocal(scale);  // (normal numbers: most is 1e-30 at least)
     const int c = column(u);
     if (c >= cols) return;
     if (u % kUnits == 0) scale_row[u / kUnits] = scale;

@@ -7,8 +7,10 @@ operators leave it in one pass over what comes before a product:
 * ``silu_mul_fp8``: ``y = g / (1 + exp(-g)) * u`` for ``x = [g | u]``, between the two products of a gated expert.
 
 Of a block of 128 columns (the last one of a row may be shorter) ``scale = max(max|y|, 1e-30) / 448`` and
-``q = e4m3(y / scale)``, rounded to nearest even; a block with a NaN in it is NaN in every place, its scale among them.
-All of it is fp32 between the loads and the one rounding of each output (csrc/fp8_rows.cu).
+``q = e4m3(y / scale)``, rounded to nearest even; a block with a NaN in it is NaN in every place, its scale among them, and
+beside an infinity what is finite is zero.
+All of it is fp32 between the loads and the one rounding of each output (csrc/fp8_rows.cu); a row whose squares add up to
+more than fp32 holds is normed to zeros.
 
 Inputs are CUDA matrices in fp16, bf16 or fp32 (all of a call of one type; the weight may be fp32 beside the others),
 with any distance between rows; rows that are not contiguous are copied first.  The operators have no gradient, in

@@ -1141,3 +1141,17 @@ def test_unsort_without_gradient_is_captured_whatever_the_weights_type():
                 refused.append(str(e))
         assert len(refused) == 1 and "eager graph" in refused[0]
         del alive
+
+
+def test_rms_norm_fp8_rows_whose_squares_leave_the_range():
+    """fp32 holds no sum of them: such a row is normed to zeros, and its neighbours are not touched."""
+    from amd_distributed_2025_b200.ops.fp8_rows import rms_norm_fp8
+
+    x = _randn(4, 264, seed=1)
+    w = torch.ones(264, device="cuda")
+    x[1] *= 1e25
+    got = rms_norm_fp8(x, w, normed=True)
+    assert bool((got.normed[1] == 0).all()) and bool((got.q[1].float() == 0).all()) and bool((got.scale[1] == got.scale[1].amin()).all())
+    for row in (0, 2, 3):
+        _check_norm(x[row:row + 1], w, None, rms_norm_fp8(x[row:row + 1], w))
+        assert torch.equal(got.q[row].view(torch.uint8), rms_norm_fp8(x[row:row + 1], w).q[0].view(torch.uint8))
