@@ -13,10 +13,10 @@ Inside an expert rows are in (token, k) order, as in the dispatch layout.  An en
 expert's are zero, in gradients too.  A token may name an expert twice and has two rows then.  Sums are fp32, over k
 upwards, rounded once; nothing depends on an order of atomics.
 
-Both are differentiable (fp16, bf16, fp32) in reverse mode; forward-mode tangents are refused.  The gradients can be had without autograd too:
-``sort_tokens_backward`` and ``unsort_tokens_backward``.  All of it may be captured into a CUDA graph; a forward pass that
-is captured while an eager graph of the same leaves is alive is refused (their gradients are added up on the eager
-graph's stream, for which a captured backward pass cannot wait).
+Both are differentiable (fp16, bf16, fp32) in reverse mode; forward-mode tangents are refused.  The gradients can be had
+without autograd too: ``sort_tokens_backward`` and ``unsort_tokens_backward``.  All of it may be captured into a CUDA graph;
+a forward pass that is captured while an eager graph of the same leaves is alive is refused (their gradients are added up on
+the eager graph's stream, for which a captured backward pass cannot wait).
 """
 from __future__ import annotations
 
